@@ -42,9 +42,9 @@ def listed():
         # A large batch with grouped keys, half-split rotation of part of the head.
         qk("head norm 32767 tokens", 32767, 32, 8, 128, 96, "half", "bf16", False, 8192),
         # One text of 8 tokens; the benchmark's batch of short texts; long texts.
-        diff("differential 8 tokens", 1, 8, 8, 6, 6, 64, "f16", -1, -1, True),
-        diff("differential 256x16-128", 256, 16, 128, 6, 6, 64, "f16", -1, -1, True),
-        diff("differential 16x2047", 16, 1024, 2047, 6, 6, 64, "bf16", -1, -1, True),
+        diff("differential 8 tokens", 1, 8, 8, 6, 6, 64, "f16", True),
+        diff("differential 256x16-128", 256, 16, 128, 6, 6, 64, "f16", True),
+        diff("differential 16x2047", 16, 1024, 2047, 6, 6, 64, "bf16", True),
     ]
 
 
@@ -61,9 +61,9 @@ def qk(name, t, hq, hk, d, rot, pairing, dt, packed, max_pos):
             "packed": packed, "max_pos": max_pos}
 
 
-def diff(name, nseq, lo, hi, h, hkv, d, dt, left, right, norm):
+def diff(name, nseq, lo, hi, h, hkv, d, dt, norm):
     return {"name": name, "op": "diff", "nseq": nseq, "lo": lo, "hi": hi, "h": h, "hkv": hkv, "d": d, "x": dt,
-            "left": left, "right": right, "norm": norm}
+            "norm": norm}
 
 
 def _log(rng, lo, hi):
@@ -99,8 +99,7 @@ def draw(rng):
             hi = _log(rng, 1, 8192)
             hkv = rng.randint(1, 6)
             c = diff("", _log(rng, 1, 512), rng.randint(max(1, hi // 8), hi), hi, hkv * rng.choice([1, 1, 2]), hkv,
-                     rng.choice([32, 64]), t, rng.choice([-1, -1, 64, 255]), rng.choice([-1, -1, 0, 64]),
-                     rng.random() < 0.7)
+                     rng.choice([32, 64]), t, rng.random() < 0.7)
             if c["nseq"] * hi * hi * c["h"] <= 16 * 2047 * 2047 * 6:
                 break
     c.pop("name")
@@ -253,11 +252,7 @@ def _plain_diff(s):
 
     q, k = heads(s["q"], 2), heads(s["k"], 2).repeat_interleave(h // hkv, 1)
     v = heads(s["v"], 1).repeat_interleave(h // hkv, 1)
-    gap = at[:, None] - at  # query minus key
-    seen = there[:, None, :] & ((gap <= c["left"]) if c["left"] >= 0 else True) & (
-        (-gap <= c["right"]) if c["right"] >= 0 else True)
-    seen = seen | (gap == 0)
-    score = (q @ k.transpose(3, 4) / math.sqrt(d)).masked_fill(~seen[:, None, None], -math.inf)
+    score = (q @ k.transpose(3, 4) / math.sqrt(d)).masked_fill(~there[:, None, None, None], -math.inf)
     p = torch.exp(score - score.amax(4, keepdim=True))
     p = p / p.sum(4, keepdim=True)
     lam = s["lam"]
@@ -303,23 +298,11 @@ def _own(s):
         return s["qo"], s["ko"]
     s["attn"].run_device(c["x"], s["q"].data_ptr(), s["k"].data_ptr(), s["v"].data_ptr(), s["offs"].data_ptr(),
                          c["nseq"], s["t"], s["max"], s["out"].data_ptr(), q_stride=s["q"].stride(0),
-                         k_stride=s["k"].stride(0), v_stride=s["v"].stride(0), window=(c["left"], c["right"]),
-                         stream=stream)
+                         k_stride=s["k"].stride(0), v_stride=s["v"].stride(0), stream=stream)
     return s["out"]
 
 
 # ------------------------------------------------------------------- work --
-
-def _pairs(c):
-    """(query, key) pairs that the windows leave, over all sequences."""
-    total = 0
-    for n in lengths(c):
-        i = np.arange(n)
-        lo = np.maximum(0, i - c["left"]) if c["left"] >= 0 else 0 * i
-        hi = np.minimum(n - 1, i + c["right"]) if c["right"] >= 0 else 0 * i + n - 1
-        total += int((hi - lo + 1).sum())
-    return total
-
 
 def work(case):
     c = case
@@ -333,7 +316,7 @@ def work(case):
         v = c["t"] * (c["hq"] + c["hk"]) * c["d"]
         return {"bytes": 2 * v * SIZE[c["x"]] + 4 * c["t"], "flops": 8 * v}
     return {"bytes": sum(lengths(c)) * (4 * c["h"] + 4 * c["hkv"]) * c["d"] * SIZE[c["x"]],
-            "flops": 12 * c["d"] * c["h"] * _pairs(c)}
+            "flops": 12 * c["d"] * c["h"] * sum(n * n for n in lengths(c))}
 
 
 # ------------------------------------------------------------------ exact --
@@ -401,16 +384,13 @@ def exact(case, seed):
     l64 = s["lam"].double()
     lam = torch.exp(l64[0] @ l64[1]) - torch.exp(l64[2] @ l64[3]) + s["init"]
     for a, b in zip(offs, offs[1:]):
-        i = torch.arange(b - a, device="cuda")
-        far = (i[:, None] - i > (c["left"] if c["left"] >= 0 else b)) | (i - i[:, None] > (
-            c["right"] if c["right"] >= 0 else b))
         for j in range(h):
             g = j // (h // c["hkv"])
             maps = []
             for part in (0, 1):
                 x = s["q"][a:b, (2 * j + part) * d:(2 * j + part + 1) * d].double()
                 y = s["k"][a:b, (2 * g + part) * d:(2 * g + part + 1) * d].double()
-                maps.append(torch.softmax((x @ y.t() * d ** -0.5).masked_fill(far, -math.inf), 1))
+                maps.append(torch.softmax(x @ y.t() * d ** -0.5, 1))
             o = (maps[0] - lam * maps[1]) @ s["v"][a:b, 2 * g * d:2 * (g + 1) * d].double()
             if s["nw"] is not None:
                 o = (1 - s["init"]) * o / (o.square().sum(1, keepdim=True) / (2 * d) + 1e-5).sqrt() * s["nw"].double()
