@@ -175,6 +175,120 @@ int le_qweight_free(le_qweight* w);
 #define LE_QGEMM_NOALLOC_MAX_ELEMS (4 * 1024 * 1024)
 int le_qgemm_device_noalloc(le_qweight* w, const float* d_x, int M, float* d_y, void* stream);
 
+/* ---------------------------------------------------------------- operators
+ * Stand-alone operators of newer encoder layers on device buffers, beside
+ * le_qgemm_device (the reference has none of them).  Each call checks its
+ * arguments on the host, enqueues its work on `stream` and returns;
+ * `stream` NULL is the handle's own stream, and (void*)1 (cudaStreamLegacy)
+ * the legacy default stream.  The caller's current device is left as it was.
+ * Calls keep nothing between them, so calls on different streams or host
+ * threads, and captured graphs, may run at the same time on buffers of their
+ * own; a call that is captured needs its buffers, workspace and handle to
+ * stay until the graph's last replay.  Element types: */
+#define LE_DT_F32 0
+#define LE_DT_F16 1
+#define LE_DT_BF16 2
+#define LE_DT_E4M3 3 /* 8-bit floating point, 4 exponent bits, no infinity */
+
+/* Quantise x [M][K] (LE_DT_F32/F16/BF16, row stride ldx elements, 0 = K) to
+ * e4m3 bytes q [M][K] with one scale for each row and 128 columns,
+ * scales [ceil(K/128)][M]: the smallest power of two (>= 2^-126) that brings
+ * the block's largest magnitude to 448 or less, 1 for a block of zeros, NaN
+ * for one that holds a NaN or an infinity.  x / scale is exact and rounded
+ * once, to nearest even.  Any M, K, stride and alignment.  On device `dev`;
+ * stream NULL is its legacy default stream. */
+int le_f8_quantize_device(int dev, int x_type, const void* d_x, int64_t ldx, int M, int K, uint8_t* d_q,
+                          float* d_scales, void* stream);
+
+/* An e4m3 weight with a scale for each block of 128 x 128:
+ *   y[m][n] = sum_b xs[b][m] ws[n/128][b] sum_{k in block b} xq[m][k] wq[n][k]
+ * with the products of a block summed on the tensor cores and the blocks in
+ * float32, rounded once to y's type.  N >= 1; K a multiple of 16 (the last
+ * block may be short). */
+typedef struct le_f8weight le_f8weight;
+/* wq [N][K] bytes and scales [ceil(N/128)][ceil(K/128)] (any float32), host
+ * or device memory (device: of `dev`, its contents complete). */
+int le_f8weight_create(int dev, const uint8_t* wq, const float* scales, int N, int K, le_f8weight** out);
+/* The same from float32 w [N][K], quantised by the rule above in blocks of
+ * 128 x 128. */
+int le_f8weight_quantize(int dev, const float* w, int N, int K, le_f8weight** out);
+/* The weight's bytes and scales back to host memory (either may be NULL). */
+int le_f8weight_read(le_f8weight* w, uint8_t* wq, float* scales);
+typedef struct {
+  const void* x;         /* [M][K] */
+  const float* x_scales; /* LE_DT_E4M3 only: [ceil(K/128)][M] as le_f8_quantize_device writes them */
+  void* y;               /* [M][N], LE_DT_F32/F16/BF16; may not overlap x */
+  void* work;            /* 16-byte aligned device memory of the call's own */
+  int64_t work_bytes;
+  int64_t ldx, ldy;      /* row strides in elements, 0 = K and N */
+  int32_t M, x_type, y_type;
+} le_f8gemm_args;
+/* Bytes of workspace that a call with M rows of x_type needs (0 for e4m3). */
+int le_f8gemm_workspace(const le_f8weight* w, int M, int x_type, int64_t* bytes);
+/* y = x . W^T.  x of LE_DT_F32/F16/BF16 is quantised within the call (any
+ * alignment and stride); x of LE_DT_E4M3 is taken as it is, 16-byte aligned
+ * with ldx a multiple of 16. */
+int le_f8gemm_device(le_f8weight* w, const le_f8gemm_args* a, void* stream);
+/* Wait for the device and report a kernel failure of an earlier call. */
+int le_f8weight_sync(le_f8weight* w);
+int le_f8weight_free(le_f8weight* w);
+
+/* Norm of query and key heads with the position rotation in the same pass:
+ *   u = x / sqrt(mean(x^2) + eps) * w over a head's columns, then
+ *   (u_a, u_b) -> (u_a c - u_b s, u_a s + u_b c) for the pairs of its first
+ * rot_dim columns, c and s of the angle position * base^(-2i / rot_dim) from a
+ * table computed in 64 bits.  Pairs: (2i, 2i+1) with LE_ROPE_INTERLEAVED (the
+ * encoder's own, ops_simd.go:127-137), (i, i + rot_dim/2) with LE_ROPE_HALF. */
+#define LE_ROPE_INTERLEAVED 0
+#define LE_ROPE_HALF 1
+typedef struct le_rope le_rope;
+/* Table of positions [0, max_pos); rot_dim even, 0 (no rotation) to 256. */
+int le_rope_create(int dev, int max_pos, int rot_dim, double base, int pairing, le_rope** out);
+typedef struct {
+  const void *q, *k;        /* token t, head h: q + t * q_stride + h * head_dim */
+  void *q_out, *k_out;      /* may be q and k themselves (with their strides); no other overlap */
+  const float *q_weight, *k_weight; /* [head_dim], NULL = ones */
+  const int32_t* positions; /* [n_tokens], in [0, max_pos); may be NULL when rot_dim is 0 */
+  int64_t q_stride, k_stride, q_out_stride, k_out_stride; /* elements between tokens, 0 = heads * head_dim */
+  int32_t type;             /* LE_DT_F32/F16/BF16 */
+  int32_t n_tokens, q_heads, k_heads; /* either number of heads may be 0 */
+  int32_t head_dim;         /* rot_dim to 256 */
+  float eps;
+} le_qk_norm_args;
+/* A token whose position lies outside the table keeps its output rows
+ * unwritten and is reported by le_rope_sync. */
+int le_qk_norm_device(le_rope* r, const le_qk_norm_args* a, void* stream);
+int le_rope_sync(le_rope* r);
+int le_rope_free(le_rope* r);
+
+/* Differential attention: the difference of two softmax maps,
+ *   o = (softmax(q1 k1^T / sqrt(d)) - lambda softmax(q2 k2^T / sqrt(d))) v
+ *   lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init
+ *   out = (1 - lambda_init) o / sqrt(mean(o^2) + eps) * norm_weight
+ * (out = o without norm_weight), every query of a sequence over all its keys.
+ * A head has two query and key parts of head_dim columns (32 or 64), side by
+ * side, and 2 * head_dim value columns; `heads` is a multiple of `kv_heads`. */
+typedef struct le_diffattn le_diffattn;
+/* lambdas: host [n_lambda][4][head_dim] as lq1, lk1, lq2, lk2, n_lambda 1 or
+ * heads; norm_weight: host [2 * head_dim] or NULL. */
+int le_diffattn_create(int dev, int heads, int kv_heads, int head_dim, const float* lambdas, int n_lambda,
+                       float lambda_init, const float* norm_weight, float eps, le_diffattn** out);
+typedef struct {
+  const void *q, *k, *v;   /* token t: q + t * q_stride, [heads][2][d]; k [kv_heads][2][d]; v [kv_heads][2d] */
+  void* out;               /* token t: out + t * out_stride, [heads][2d]; may not overlap the inputs */
+  const int32_t* offsets;  /* device [nseq + 1], ascending within [0, n_tokens]: sequence s has rows
+                            * offsets[s] .. offsets[s+1); rows outside are neither read nor written */
+  int64_t q_stride, k_stride, v_stride, out_stride; /* elements, multiples of 8; 0 = packed */
+  int32_t type;            /* LE_DT_F16 or LE_DT_BF16; pointers 16-byte aligned */
+  int32_t nseq, n_tokens;
+  int32_t max_len;         /* longest sequence if known, else 0: only chooses the kernel */
+} le_diffattn_args;
+/* Offsets that descend or leave [0, n_tokens] are reported by
+ * le_diffattn_sync; their sequences are not computed. */
+int le_diffattn_device(le_diffattn* h, const le_diffattn_args* a, void* stream);
+int le_diffattn_sync(le_diffattn* h);
+int le_diffattn_free(le_diffattn* h);
+
 /* Per-kernel device timing of le_embed_ids / le_embed_ids_device calls.
  * With profiling on, every kernel launch of the forward pass is bracketed by
  * CUDA events on its stream; le_get_stats synchronises and returns the

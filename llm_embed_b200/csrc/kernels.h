@@ -118,4 +118,54 @@ cudaError_t launch_gemm_ln(const __half* W16, int K, const __half* A, long lda, 
 cudaError_t launch_gemm_f16(const __half* W16, int n_virtual, int K, const __half* A, long lda, const EpiParams& ep,
                             DevStatus* status, cudaStream_t s);
 
+// qk_norm.cu: per-head norm of queries and keys with the rotation.
+struct QkNormParams {
+  const void *q, *k;
+  void *q_out, *k_out;
+  long q_stride, k_stride, qo_stride, ko_stride;  // elements between tokens
+  int q_heads, k_heads, d, rot, half_split, max_pos;
+  const float *q_weight, *k_weight;  // [d] or null
+  const float *cos, *sin;            // [max_pos][rot/2]
+  const int32_t* positions;          // [n_tokens] or null (rot 0)
+  float eps;
+  DevStatus* status;
+  // set by the launcher
+  int token0;
+  uint32_t items, inv_heads;
+};
+cudaError_t launch_qk_norm(int dt, QkNormParams p, int n_tokens, cudaStream_t s);
+cudaError_t launch_rope_table(int max_pos, int rot, double base, float* cos, float* sin, cudaStream_t s);
+
+// f8_quant.cu
+cudaError_t launch_f8_quantize(int dt, const void* x, long ldx, int M, int K, uint8_t* q, float* scales,
+                               cudaStream_t s);
+cudaError_t launch_f8_quantize_weight(const float* w, int N, int K, uint8_t* q, float* scales, cudaStream_t s);
+
+// f8_gemm.cu: the e4m3 product with a scale per block of 128.  K is a
+// multiple of 16 and x rows are 16-byte aligned.
+struct F8GemmParams {
+  const void* x;      // [M][K], row stride ldx (elements)
+  const float* xs;    // [ceil(K/128)][M] scales of e4m3 activations
+  const uint8_t* w;   // [N][K] e4m3
+  const float* ws;    // [ceil(N/128)][ceil(K/128)]
+  void* y;            // [M][N], row stride ldy
+  long ldx, ldy;
+  int M, N, K;
+};
+cudaError_t launch_f8_gemm_small(int xdt, int ydt, const F8GemmParams& p, cudaStream_t s);
+
+// diff_attention.cu: differential attention over packed sequences.
+struct DiffParams {
+  const void *q, *k, *v;  // [T][H][2][d], [T][Hkv][2][d], [T][Hkv][2d]
+  void* out;              // [T][H][2d]
+  long q_stride, k_stride, v_stride, o_stride;  // elements between tokens
+  const int32_t* offsets;  // [nseq + 1]
+  int nseq, T, heads, group;  // group: query heads per key head
+  const float* lambda;     // [heads]
+  const float* norm_w;     // [2d] or null
+  float out_scale, eps;    // 1 - lambda_init
+  DevStatus* status;
+};
+cudaError_t launch_diff_attention(int dt, int d, const DiffParams& p, cudaStream_t s);
+
 }  // namespace le
