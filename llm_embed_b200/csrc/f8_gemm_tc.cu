@@ -1,0 +1,416 @@
+// Eight-bit product on the tensor cores (tcgen05 kind::f8f6f4, sm_100a):
+//   y[m][n] = sum_b xs[b][m] ws[n/128][b] sum_{k in block b} xq[m][k] wq[n][k]
+//
+// The weight's scales are any float32, so they cannot be left to the MMA's
+// own power-of-two scaling: each K block of 128 is one accumulator of its own
+// in TMEM (four MMAs of K = 32, the first overwriting), and the epilogue warps
+// add it, times the row's and the weight block's scale, to float32 sums in
+// registers while the tensor cores fill the other accumulators.  A thread
+// holds one row's columns of one weight block, so a block costs it one
+// multiplier and half a packed fma per column.
+//
+// Persistent kernel; tile = 128 * CG token rows x BN weight rows.  CG = 2: a
+// cluster of two CTAs computes it with one MMA of M = 256 (cta_group::2), each
+// CTA loading its 128 token rows and half of the weight rows.
+//   warp 0     producer: TMA loads, one K block (128 bytes a row, 128B
+//              swizzle) per stage
+//   warp 1     TMEM allocation; one lane (of the even CTA) issues the MMAs
+//   warps 4-   epilogue: TMEM lanes by warp % 4, columns by group of four;
+//              rows go out through shared memory and TMA stores, or by plain
+//              stores where y's rows do not begin and end on 16 bytes
+// Rows and columns past M, N and K are zeros from TMA and are not stored.
+// Every mbarrier wait is bounded (WAIT_LIMIT_NS).
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "elem.cuh"
+#include "gemm_epi_tc.cuh"
+#include "kernels.h"
+#include "tcgen05.cuh"
+
+namespace le {
+namespace f8t {
+
+using namespace tcx;
+
+constexpr int BM = 128;
+constexpr int BK = 128;  // one scale block
+constexpr int EPI_WARP0 = 4;
+
+template <int CG, int BN, int STAGES, int NACC>
+struct Cfg {
+  static constexpr int cg = CG, bn = BN, stages = STAGES, nacc = NACC;
+  // Two groups of four epilogue warps share the columns of the wider tiles; a
+  // group has at least 64 (a 128-byte row of a 16-bit result).
+  static constexpr int EPI_WARPS = BN >= 128 ? 8 : 4;
+  static constexpr int COLS = BN / (EPI_WARPS / 4);  // columns of a warp
+  static constexpr int NTHREADS = (EPI_WARP0 + EPI_WARPS) * 32;
+  static constexpr int B_ROWS = BN / CG;  // weight rows per CTA
+  static constexpr int A_BYTES = BM * BK, B_BYTES = B_ROWS * BK;
+  static constexpr int OFF_A = 0;
+  static constexpr int OFF_B = OFF_A + STAGES * A_BYTES;
+  static constexpr int OFF_STAGE = OFF_B + STAGES * B_BYTES;
+  static constexpr int OFF_BAR = OFF_STAGE + EPI_WARPS * 2 * 4096;
+  static constexpr int NBAR = 2 * STAGES + 2 * NACC;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int ALLOC = OFF_MISC + 16 + 1024;
+  static constexpr int TMEM_COLS = NACC * BN;
+  static_assert(ALLOC <= 232448, "shared memory of one CTA");
+  static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "TMEM columns");
+};
+
+template <int CG>
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 2)
+    mma_commit_pair(bar, 0x3);
+  else
+    mma_commit(bar);
+}
+
+// Plain stores of 32 rows x 32 columns staged in the warp's shared memory:
+// consecutive lanes write consecutive columns of a row.
+template <class Y>
+__device__ __forceinline__ void store_plain(float* stg, const float* v, Y* y, long ldy, int row0, int col0, int M,
+                                            int N) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 32; j++) stg[lane * 33 + j] = v[j];
+  __syncwarp();
+  if (col0 + lane < N) {
+    const int n = min(32, M - row0);
+    for (int i = 0; i < n; i++) y[(long)(row0 + i) * ldy + col0 + lane] = from_f32<Y>(stg[i * 33 + lane]);
+  }
+  __syncwarp();
+}
+
+template <class C, class Y>
+__global__ void __launch_bounds__(C::NTHREADS, 1)
+    f8_tc_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                 const __grid_constant__ CUtensorMap tmap_y, int use_tma, F8GemmParams p, int m_tiles, int n_tiles,
+                 DevStatus* status) {
+  constexpr int CG = C::cg, BN = C::bn, S = C::stages, NACC = C::nacc, COLS = C::COLS, EPI_WARPS = C::EPI_WARPS;
+  constexpr uint32_t IDESC = idesc_f16(CG * BM, BN);  // e4m3 x e4m3 has the same type fields (0)
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + C::OFF_BAR;
+  auto full = [&](int s) { return bar0 + 8 * s; };
+  auto empty = [&](int s) { return bar0 + 8 * (S + s); };
+  auto tfull = [&](int a) { return bar0 + 8 * (2 * S + a); };
+  auto tempty = [&](int a) { return bar0 + 8 * (2 * S + NACC + a); };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
+  const bool leader = rank == 0;
+  const int KB = (p.K + BK - 1) / BK;
+  const int total = m_tiles * n_tiles;
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < S; s++) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < NACC; a++) {
+      mbar_init(tfull(a), 1);
+      mbar_init(tempty(a), CG * EPI_WARPS);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(C::TMEM_COLS));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(C::TMEM_COLS));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // both CTAs' barriers are initialised before any remote arrive
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();  // the quantised activations are the previous kernel's
+  pdl_trigger();
+  // The widest tile's epilogue holds 128 sums a thread: of the 384 x 168
+  // registers at launch the first warpgroup keeps 40 each, the two of the
+  // epilogue take 232.
+  if (warp < EPI_WARP0) {
+  if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_a)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_b)) : "memory");
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += step) {
+        const int mt = tile / n_tiles, nt = tile % n_tiles;
+        const int row = (mt * CG + (int)rank) * BM, col = nt * BN + (int)rank * C::B_ROWS;
+        for (int kb = 0; kb < KB; kb++, it++) {
+          const int s = it % S;
+          if (!mbar_wait(empty(s), ((it / S) & 1) ^ 1, abort_flag, status, 50)) {
+            ok = false;
+            break;
+          }
+          if (leader) mbar_expect_tx(full(s), CG * (C::A_BYTES + C::B_BYTES));
+          const uint32_t a = sbase + C::OFF_A + s * C::A_BYTES, b = sbase + C::OFF_B + s * C::B_BYTES;
+          if constexpr (CG == 2) {
+            const uint32_t bar = map_to_rank(full(s), 0);
+            tma_load_2d_pair(a, &tmap_a, kb * BK, row, bar);
+            tma_load_2d_pair(b, &tmap_b, kb * BK, col, bar);
+          } else {
+            tma_load_2d(a, &tmap_a, kb * BK, row, full(s));
+            tma_load_2d(b, &tmap_b, kb * BK, col, full(s));
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA
+    if (leader && lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += step) {
+        for (int kb = 0; kb < KB; kb++, it++) {
+          const int s = it % S, acc = it % NACC;
+          if (!mbar_wait(tempty(acc), ((it / NACC) & 1) ^ 1, abort_flag, status, 51) ||
+              !mbar_wait(full(s), (it / S) & 1, abort_flag, status, 52)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = sbase + C::OFF_A + s * C::A_BYTES, b = sbase + C::OFF_B + s * C::B_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < BK / 32; kk++)
+            mma_f8<CG>(tmem + acc * BN, sw128_desc(a + kk * 32), sw128_desc(b + kk * 32), IDESC, kk != 0);
+          commit<CG>(empty(s));
+          commit<CG>(tfull(acc));
+        }
+      }
+    }
+  }
+  } else {
+    if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp & 3, ew = warp - EPI_WARP0;
+    const int c0 = (ew >> 2) * COLS;  // this warp's columns of the tile
+    const uint32_t stage = sbase + C::OFF_STAGE + ew * 2 * 4096;
+    float* stg = reinterpret_cast<float*>(smem + C::OFF_STAGE + ew * 2 * 4096);
+    int buf = 0;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int tile = first; tile < total && ok; tile += step) {
+      const int mt = tile / n_tiles, nt = tile % n_tiles;
+      const int row0 = (mt * CG + (int)rank) * BM + quarter * 32;
+      const int n0 = nt * BN + c0;
+      // Clamped rows and columns read a scale that exists and are not stored.
+      const float* xs = p.xs + min(row0 + lane, p.M - 1);
+      const float* ws = p.ws + (long)(min(n0, p.N - 1) / 128) * KB;
+      unsigned long long acc[COLS / 2];
+#pragma unroll
+      for (int i = 0; i < COLS / 2; i++) acc[i] = 0;
+      float next = __ldg(xs) * __ldg(ws);
+      for (int kb = 0; kb < KB; kb++, it++) {
+        const int a = it % NACC;
+        const float sc = next;
+        if (kb + 1 < KB) next = __ldg(xs + (long)(kb + 1) * p.M) * __ldg(ws + kb + 1);
+        if (!__all_sync(0xffffffffu, mbar_wait(tfull(a), (it / NACC) & 1, abort_flag, status, 53))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const unsigned long long sc2 = f2_pack(sc, sc);
+        const uint32_t t = tmem + a * BN + c0 + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) {
+          float v[32];
+          tmem_ld32(t + c, v);
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            acc[c / 2 + i] = f2_fma(f2_pack(v[2 * i], v[2 * i + 1]), sc2, acc[c / 2 + i]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2)
+            mbar_arrive_cluster(map_to_rank(tempty(a), 0));
+          else
+            mbar_arrive(tempty(a));
+        }
+      }
+      if (!ok) break;
+      if (row0 >= p.M) continue;  // warp-uniform
+      if (use_tma) {
+        constexpr int PER = 128 / sizeof(Y);  // columns of a 128-byte block
+#pragma unroll
+        for (int c = 0; c < COLS; c += PER) {
+          if (n0 + c >= p.N) break;
+          uint32_t words[32];
+#pragma unroll
+          for (int i = 0; i < PER / 2; i++) {
+            float lo, hi;
+            f2_unpack(acc[c / 2 + i], lo, hi);
+            if constexpr (sizeof(Y) == 4) {
+              words[2 * i] = __float_as_uint(lo);
+              words[2 * i + 1] = __float_as_uint(hi);
+            } else {
+              words[i] = pack2<Y>(lo, hi);
+            }
+          }
+          emit_block(&tmap_y, stage, buf, words, n0 + c, row0);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) {
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 16; i++) f2_unpack(acc[c / 2 + i], v[2 * i], v[2 * i + 1]);
+          store_plain<Y>(stg, v, static_cast<Y*>(p.y), p.ldy, row0, n0 + c, p.M, p.N);
+        }
+      }
+    }
+    if (use_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the peer is done with this CTA's shared memory and TMEM
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (CG == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS));
+  }
+}
+
+// ---------------------------------------------------------------- host ----
+
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// 2-D row-major map of bytes_per-element elements with 128B-swizzled boxes.
+static bool encode(PFN_cuTensorMapEncodeTiled_v12000 enc, CUtensorMap* map, CUtensorMapDataType type, int esz,
+                   const void* p, long rows, long cols, long ld, int box_cols, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * esz};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(map, type, 2, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class C, class Y>
+static cudaError_t launch(int ydt, const F8GemmParams& p, DevStatus* status, cudaStream_t s) {
+  auto enc = encode_fn();
+  if (!enc) return cudaErrorNotSupported;
+  CUtensorMap amap, bmap, ymap = {};
+  if (!encode(enc, &amap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.x, p.M, p.K, p.ldx, BK, BM) ||
+      !encode(enc, &bmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.N, p.K, p.K, BK, C::B_ROWS))
+    return cudaErrorInvalidValue;
+  // A TMA store clips the last columns at 16-byte steps only, so N must end on
+  // one for the columns behind to stay as they were.
+  const int use_tma = reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && (p.ldy * (long)sizeof(Y)) % 16 == 0 &&
+                      (p.N * (long)sizeof(Y)) % 16 == 0;
+  const CUtensorMapDataType yt = ydt == DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : ydt == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (use_tma && !encode(enc, &ymap, yt, sizeof(Y), p.y, p.M, p.N, p.ldy, 128 / sizeof(Y), 32))
+    return cudaErrorInvalidValue;
+  // Per device: the shared-memory attribute and how many clusters fit at once.
+  static std::mutex mu;
+  static int resident[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64) return cudaErrorInvalidDevice;
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C::cg;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (resident[dev] == 0) {
+      cudaError_t e = cudaFuncSetAttribute(f8_tc_kernel<C, Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::ALLOC);
+      if (e != cudaSuccess) return e;
+      int sms = 0, n = 0;
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(sms / C::cg * C::cg);
+      cfg.blockDim = dim3(C::NTHREADS);
+      cfg.dynamicSmemBytes = C::ALLOC;
+      cfg.attrs = attr + 1;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&n, f8_tc_kernel<C, Y>, &cfg);
+      if (e != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        n = sms / C::cg;
+      }
+      resident[dev] = n;
+    }
+  }
+  const int m_tiles = (p.M + C::cg * BM - 1) / (C::cg * BM), n_tiles = (p.N + C::bn - 1) / C::bn;
+  const long total = (long)m_tiles * n_tiles;
+  if (total > 0x7fffffff) return cudaErrorInvalidValue;
+  const int clusters = total < resident[dev] ? (int)total : resident[dev];
+  cudaLaunchConfig_t cfg = pdl_config(dim3(clusters * C::cg), dim3(C::NTHREADS), C::ALLOC, s, attr);
+  cfg.numAttrs = C::cg == 2 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, f8_tc_kernel<C, Y>, amap, bmap, ymap, use_tma, p, m_tiles, n_tiles, status);
+}
+
+using Pair = Cfg<2, 256, 5, 2>;
+using Tile128 = Cfg<1, 128, 4, 4>;
+using Tile64 = Cfg<1, 64, 4, 4>;
+
+template <class Y>
+static cudaError_t pick(int ydt, const F8GemmParams& p, DevStatus* status, cudaStream_t s) {
+  const long mt = (p.M + 127) / 128;
+  // Pairs of 256 x 256 once they fill the 74 pairs of SMs; below that the
+  // widest tile that gives every SM one.
+  if ((mt + 1) / 2 * ((p.N + 255) / 256) >= 74) return launch<Pair, Y>(ydt, p, status, s);
+  if (mt * ((p.N + 127) / 128) >= 148) return launch<Tile128, Y>(ydt, p, status, s);
+  return launch<Tile64, Y>(ydt, p, status, s);
+}
+
+}  // namespace f8t
+
+cudaError_t launch_f8_gemm_tc(int ydt, const F8GemmParams& p, DevStatus* status, cudaStream_t s) {
+  if (p.M == 0) return cudaSuccess;
+  return ydt == DT_F32   ? f8t::pick<float>(ydt, p, status, s)
+         : ydt == DT_F16 ? f8t::pick<__half>(ydt, p, status, s)
+                         : f8t::pick<__nv_bfloat16>(ydt, p, status, s);
+}
+
+}  // namespace le

@@ -153,6 +153,8 @@ struct F8GemmParams {
   int M, N, K;
 };
 cudaError_t launch_f8_gemm_small(int xdt, int ydt, const F8GemmParams& p, cudaStream_t s);
+// f8_gemm_tc.cu: e4m3 activations, tcgen05 tiles.
+cudaError_t launch_f8_gemm_tc(int ydt, const F8GemmParams& p, DevStatus* status, cudaStream_t s);
 
 // diff_attention.cu: differential attention over packed sequences.
 struct DiffParams {
