@@ -81,6 +81,27 @@ __device__ __forceinline__ void commit(uint32_t bar) {
     mma_commit(bar);
 }
 
+// 32 TMEM columns of the warp's lanes; the registers hold them after wait_ld,
+// which names them so that no use moves above it.
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%"
+      "20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
 // Plain stores of 32 rows x 32 columns staged in the warp's shared memory:
 // consecutive lanes write consecutive columns of a row.
 template <class Y>
@@ -230,11 +251,22 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       unsigned long long acc[COLS / 2];
 #pragma unroll
       for (int i = 0; i < COLS / 2; i++) acc[i] = 0;
-      float next = __ldg(xs) * __ldg(ws);
+      // Scales are loaded two blocks ahead and multiplied when needed: a block
+      // takes less time than a load from L2.
+      float x0 = __ldg(xs), w0 = __ldg(ws), x1 = 0.f, w1 = 0.f;
+      if (KB > 1) {
+        x1 = __ldg(xs + p.M);
+        w1 = __ldg(ws + 1);
+      }
       for (int kb = 0; kb < KB; kb++, it++) {
         const int a = it % NACC;
-        const float sc = next;
-        if (kb + 1 < KB) next = __ldg(xs + (long)(kb + 1) * p.M) * __ldg(ws + kb + 1);
+        const float sc = x0 * w0;
+        x0 = x1;
+        w0 = w1;
+        if (kb + 2 < KB) {
+          x1 = __ldg(xs + (long)(kb + 2) * p.M);
+          w1 = __ldg(ws + kb + 2);
+        }
         if (!__all_sync(0xffffffffu, mbar_wait(tfull(a), (it / NACC) & 1, abort_flag, status, 53))) {
           ok = false;
           break;
@@ -242,13 +274,18 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         tc_fence_after();
         const unsigned long long sc2 = f2_pack(sc, sc);
         const uint32_t t = tmem + a * BN + c0 + ((uint32_t)(quarter * 32) << 16);
+        // The next 32 columns are on their way while these are added.
+        uint32_t v[2][32];
+        ld32(t, v[0]);
 #pragma unroll
         for (int c = 0; c < COLS; c += 32) {
-          float v[32];
-          tmem_ld32(t + c, v);
+          uint32_t(&u)[32] = v[(c / 32) & 1];
+          wait_ld(u);
+          if (c + 32 < COLS) ld32(t + c + 32, v[(c / 32 + 1) & 1]);
 #pragma unroll
           for (int i = 0; i < 16; i++)
-            acc[c / 2 + i] = f2_fma(f2_pack(v[2 * i], v[2 * i + 1]), sc2, acc[c / 2 + i]);
+            acc[c / 2 + i] = f2_fma(f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), sc2,
+                                    acc[c / 2 + i]);
         }
         tc_fence_before();
         __syncwarp();
