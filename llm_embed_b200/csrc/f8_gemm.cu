@@ -20,7 +20,6 @@ namespace f8s {
 
 using namespace f8;
 
-constexpr int WARPS = 8;
 constexpr int ROWS = 16;  // weight rows per CTA
 
 struct E4m3 {};  // activations that are quantised already
@@ -38,25 +37,20 @@ __device__ __forceinline__ uint4 ldw(const uint8_t* p, bool ok) {
   return ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
 }
 
-// This lane's 32 activations of block kb of token m, as fragments, and the
-// block's scale.  Columns from K on are zero.
+// This lane's 32 activations of block kb of token m as they lie in memory
+// (zero from column K and row M on), and as fragments with the block's scale.
 template <class X>
-__device__ __forceinline__ float act_frag(const F8GemmParams& p, int m, int kb, int t, uint32_t (&b)[8]) {
-  const int k0 = kb * BLOCK + 16 * t;
-  const bool row = m < p.M;
-  if constexpr (sizeof(X) == 1) {
-    const uint8_t* x = static_cast<const uint8_t*>(p.x) + (long)m * p.ldx;
-#pragma unroll
-    for (int c = 0; c < 2; c++) *reinterpret_cast<uint4*>(b + 4 * c) = ldw(x + k0 + 64 * c, row && k0 + 64 * c < p.K);
-    return row ? __ldg(p.xs + (long)kb * p.M + m) : 0.f;
-  } else {
+struct Act {
+  Raw8<X> raw[4];
+  __device__ __forceinline__ void load(const F8GemmParams& p, int m, int kb, int t) {
     const X* x = static_cast<const X*>(p.x) + (long)m * p.ldx;
-    Raw8<X> raw[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const int k = k0 + 64 * (i >> 1) + 8 * (i & 1);
-      raw[i] = row && k < p.K ? load8(x + k) : zero8<X>();
+      const int k = kb * BLOCK + 16 * t + 64 * (i >> 1) + 8 * (i & 1);
+      raw[i] = m < p.M && k < p.K ? load8(x + k) : zero8<X>();
     }
+  }
+  __device__ __forceinline__ float frag(uint32_t (&b)[8]) const {
     uint32_t a = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -78,80 +72,128 @@ __device__ __forceinline__ float act_frag(const F8GemmParams& p, int m, int kb, 
     }
     return s;
   }
-}
-
-template <class X, class Y, int NT>
-__global__ void __launch_bounds__(WARPS * 32) f8_small_kernel(F8GemmParams p) {
-  pdl_wait();
-  pdl_trigger();
-  __shared__ float red[WARPS][NT * 8][ROWS + 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * ROWS, m0 = blockIdx.y * (8 * NT);
-  const int KB = (p.K + BLOCK - 1) / BLOCK;
-  const float* ws = p.ws + (long)(n0 / BLOCK) * KB;
-  const uint8_t* wa = p.w + (long)(n0 + g) * p.K;
-  const uint8_t* wb = wa + 8L * p.K;
-  const bool ra = n0 + g < p.N, rb = n0 + g + 8 < p.N;
-  float acc[NT][4];
-#pragma unroll
-  for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-#pragma unroll 2
-  for (int kb = warp; kb < KB; kb += WARPS) {
-    uint4 a[2], b[2];
+};
+template <>
+struct Act<E4m3> {
+  uint4 raw[2];
+  float scale;
+  __device__ __forceinline__ void load(const F8GemmParams& p, int m, int kb, int t) {
+    const uint8_t* x = static_cast<const uint8_t*>(p.x) + (long)m * p.ldx;
 #pragma unroll
     for (int c = 0; c < 2; c++) {
-      const int k = kb * BLOCK + 64 * c + 16 * t;
-      a[c] = ldw(wa + k, ra && k < p.K);
-      b[c] = ldw(wb + k, rb && k < p.K);
+      const int k = kb * BLOCK + 16 * t + 64 * c;
+      raw[c] = m < p.M && k < p.K ? *reinterpret_cast<const uint4*>(x + k) : make_uint4(0, 0, 0, 0);
     }
-    const float wsc = __ldg(ws + kb);
+    scale = m < p.M && kb * BLOCK < p.K ? p.xs[(long)kb * p.M + m] : 0.f;
+  }
+  __device__ __forceinline__ float frag(uint32_t (&b)[8]) const {
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-      uint32_t f[8];
-      const float xs = act_frag<X>(p, m0 + 8 * j + g, kb, t, f);
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < 2; c++) *reinterpret_cast<uint4*>(b + 4 * c) = raw[c];
+    return scale;
+  }
+};
+
+// NT groups of eight tokens, RT tiles of 16 weight rows per CTA, DEPTH K
+// blocks of each warp in flight.
+template <class X, class Y, int NT, int RT, int DEPTH, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) f8_small_kernel(F8GemmParams p) {
+  __shared__ float red[WARPS][NT * 8][RT * ROWS + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * (RT * ROWS), m0 = blockIdx.y * (8 * NT);
+  const int KB = (p.K + BLOCK - 1) / BLOCK;
+  const float* ws = p.ws + (long)(n0 / BLOCK) * KB;
+  const uint8_t* wrow = p.w + (long)(n0 + g) * p.K;
+  uint4 w[DEPTH][2 * RT][2];
+  float wsc[DEPTH];
+  // Rows g, g + 8, .. of block kb: two pieces of 16 bytes each.
+  auto load_w = [&](int d, int kb) {
+#pragma unroll
+    for (int r = 0; r < 2 * RT; r++)
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        mma_e4m3(d, a[c].x, b[c].x, a[c].y, b[c].y, f[4 * c], f[4 * c + 1]);
-        mma_e4m3(d, a[c].z, b[c].z, a[c].w, b[c].w, f[4 * c + 2], f[4 * c + 3]);
+        const int k = kb * BLOCK + 64 * c + 16 * t;
+        w[d][r][c] = ldw(wrow + (long)(8 * r) * p.K + k, n0 + g + 8 * r < p.N && k < p.K);
       }
-      // Columns 2t and 2t + 1 of the result: the scales of those tokens.
-      const float s0 = __shfl_sync(0xffffffffu, xs, 8 * t) * wsc, s1 = __shfl_sync(0xffffffffu, xs, 8 * t + 4) * wsc;
-      acc[j][0] = fmaf(d[0], s0, acc[j][0]);
-      acc[j][1] = fmaf(d[1], s1, acc[j][1]);
-      acc[j][2] = fmaf(d[2], s0, acc[j][2]);
-      acc[j][3] = fmaf(d[3], s1, acc[j][3]);
+    wsc[d] = kb < KB ? __ldg(ws + kb) : 0.f;
+  };
+  // The weight is no other kernel's result, so its first blocks are under way
+  // before the previous kernel (the quantiser, if there is one) has ended.
+#pragma unroll
+  for (int d = 0; d < DEPTH; d++) load_w(d, warp + d * WARPS);
+  pdl_wait();
+  pdl_trigger();
+  float acc[RT][NT][4];
+#pragma unroll
+  for (int r = 0; r < RT; r++)
+#pragma unroll
+    for (int j = 0; j < NT; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0.f;
+  for (int kb0 = warp; kb0 < KB; kb0 += WARPS * DEPTH) {
+    Act<X> x[DEPTH][NT];
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) x[d][j].load(p, m0 + 8 * j + g, kb0 + d * WARPS, t);
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) {
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        uint32_t f[8];
+        const float xs = x[d][j].frag(f);
+        // Columns 2t and 2t + 1 of the result: the scales of those tokens.
+        const float s0 = __shfl_sync(0xffffffffu, xs, 8 * t) * wsc[d];
+        const float s1 = __shfl_sync(0xffffffffu, xs, 8 * t + 4) * wsc[d];
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const uint4 a = w[d][2 * r][c], b = w[d][2 * r + 1][c];
+            mma_e4m3(v, a.x, b.x, a.y, b.y, f[4 * c], f[4 * c + 1]);
+            mma_e4m3(v, a.z, b.z, a.w, b.w, f[4 * c + 2], f[4 * c + 3]);
+          }
+          acc[r][j][0] = fmaf(v[0], s0, acc[r][j][0]);
+          acc[r][j][1] = fmaf(v[1], s1, acc[r][j][1]);
+          acc[r][j][2] = fmaf(v[2], s0, acc[r][j][2]);
+          acc[r][j][3] = fmaf(v[3], s1, acc[r][j][3]);
+        }
+      }
+      load_w(d, kb0 + (DEPTH + d) * WARPS);
     }
   }
 #pragma unroll
-  for (int j = 0; j < NT; j++) {
-    red[warp][8 * j + 2 * t][g] = acc[j][0];
-    red[warp][8 * j + 2 * t + 1][g] = acc[j][1];
-    red[warp][8 * j + 2 * t][g + 8] = acc[j][2];
-    red[warp][8 * j + 2 * t + 1][g + 8] = acc[j][3];
-  }
+  for (int r = 0; r < RT; r++)
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      red[warp][8 * j + 2 * t][r * ROWS + g] = acc[r][j][0];
+      red[warp][8 * j + 2 * t + 1][r * ROWS + g] = acc[r][j][1];
+      red[warp][8 * j + 2 * t][r * ROWS + g + 8] = acc[r][j][2];
+      red[warp][8 * j + 2 * t + 1][r * ROWS + g + 8] = acc[r][j][3];
+    }
   __syncthreads();
-  for (int i = threadIdx.x; i < NT * 8 * ROWS; i += WARPS * 32) {
-    const int m = i / ROWS, n = i % ROWS;
+  for (int i = threadIdx.x; i < NT * 8 * RT * ROWS; i += WARPS * 32) {
+    const int m = i / (RT * ROWS), n = i % (RT * ROWS);
     float v = red[0][m][n];
 #pragma unroll
-    for (int w = 1; w < WARPS; w++) v += red[w][m][n];
+    for (int k = 1; k < WARPS; k++) v += red[k][m][n];
     if (m0 + m < p.M && n0 + n < p.N) static_cast<Y*>(p.y)[(long)(m0 + m) * p.ldy + n0 + n] = from_f32<Y>(v);
   }
 }
 
-template <class X, class Y, int NT>
+template <class X, class Y, int NT, int RT, int DEPTH, int WARPS>
 static cudaError_t launch_nt(const F8GemmParams& p, cudaStream_t s) {
   cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg = pdl_config(dim3((p.N + ROWS - 1) / ROWS, (p.M + 8 * NT - 1) / (8 * NT)),
-                                            dim3(WARPS * 32), 0, s, attr);
-  return cudaLaunchKernelEx(&cfg, f8_small_kernel<X, Y, NT>, p);
+  const cudaLaunchConfig_t cfg = pdl_config(
+      dim3((p.N + RT * ROWS - 1) / (RT * ROWS), (p.M + 8 * NT - 1) / (8 * NT)), dim3(WARPS * 32), 0, s, attr);
+  return cudaLaunchKernelEx(&cfg, f8_small_kernel<X, Y, NT, RT, DEPTH, WARPS>, p);
 }
 template <class X, class Y>
 static cudaError_t launch_xy(const F8GemmParams& p, cudaStream_t s) {
-  if (p.M <= 8) return launch_nt<X, Y, 1>(p, s);
-  if (p.M <= 16) return launch_nt<X, Y, 2>(p, s);
-  return launch_nt<X, Y, 4>(p, s);
+  if constexpr (sizeof(X) == 1) {
+    if (p.M > 24) return launch_nt<X, Y, 4, 1, 1, 8>(p, s);
+    if (p.M > 16) return launch_nt<X, Y, 3, 1, 1, 8>(p, s);
+    if (p.M > 8) return launch_nt<X, Y, 2, 1, 1, 8>(p, s);
+  }
+  return launch_nt<X, Y, 1, 1, 1, 8>(p, s);
 }
 template <class X>
 static cudaError_t launch_x(int ydt, const F8GemmParams& p, cudaStream_t s) {

@@ -73,6 +73,11 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+  return e != 0;
+}
 template <int CG>
 __device__ __forceinline__ void commit(uint32_t bar) {
   if constexpr (CG == 2)
@@ -209,24 +214,30 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA
-    if (leader && lane == 0) {
+    // The whole warp walks the loop, so that its addresses are uniform; one
+    // lane issues.
+    if (leader) {
+      const bool issuer = elect_one();
+      const uint64_t a0 = sw128_desc(sbase + C::OFF_A), b0 = sw128_desc(sbase + C::OFF_B);
       uint32_t it = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += step) {
-        for (int kb = 0; kb < KB; kb++, it++) {
-          const int s = it % S, acc = it % NACC;
-          if (!mbar_wait(tempty(acc), ((it / NACC) & 1) ^ 1, abort_flag, status, 51) ||
-              !mbar_wait(full(s), (it / S) & 1, abort_flag, status, 52)) {
-            ok = false;
-            break;
-          }
+        for (int kb = 0; kb < KB && ok; kb++, it++) {
+          const uint32_t s = it % S, acc = it % NACC;
+          ok = mbar_wait(full(s), (it / S) & 1, abort_flag, status, 52) &&
+               mbar_wait(tempty(acc), ((it / NACC) & 1) ^ 1, abort_flag, status, 51);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a = sbase + C::OFF_A + s * C::A_BYTES, b = sbase + C::OFF_B + s * C::B_BYTES;
+          if (issuer) {
+            // Descriptor addresses count 16-byte units.
+            const uint64_t a = a0 + s * (C::A_BYTES / 16), b = b0 + s * (C::B_BYTES / 16);
 #pragma unroll
-          for (int kk = 0; kk < BK / 32; kk++)
-            mma_f8<CG>(tmem + acc * BN, sw128_desc(a + kk * 32), sw128_desc(b + kk * 32), IDESC, kk != 0);
-          commit<CG>(empty(s));
-          commit<CG>(tfull(acc));
+            for (int kk = 0; kk < BK / 32; kk++) mma_f8<CG>(tmem + acc * BN, a + kk * 2, b + kk * 2, IDESC, kk != 0);
+            commit<CG>(tfull(acc));
+            commit<CG>(empty(s));
+          }
+          __syncwarp();
         }
       }
     }
@@ -241,23 +252,29 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     int buf = 0;
     uint32_t it = 0;
     bool ok = true;
-    for (int tile = first; tile < total && ok; tile += step) {
-      const int mt = tile / n_tiles, nt = tile % n_tiles;
-      const int row0 = (mt * CG + (int)rank) * BM + quarter * 32;
-      const int n0 = nt * BN + c0;
+    // Scales are loaded two blocks ahead and multiplied when needed: a block
+    // takes less time than a load from L2.
+    const float *xs, *ws;
+    float x0 = 0.f, w0 = 0.f, x1 = 0.f, w1 = 0.f;
+    auto first_scales = [&](int tile) {
+      if (tile >= total) return;
       // Clamped rows and columns read a scale that exists and are not stored.
-      const float* xs = p.xs + min(row0 + lane, p.M - 1);
-      const float* ws = p.ws + (long)(min(n0, p.N - 1) / 128) * KB;
-      unsigned long long acc[COLS / 2];
-#pragma unroll
-      for (int i = 0; i < COLS / 2; i++) acc[i] = 0;
-      // Scales are loaded two blocks ahead and multiplied when needed: a block
-      // takes less time than a load from L2.
-      float x0 = __ldg(xs), w0 = __ldg(ws), x1 = 0.f, w1 = 0.f;
+      xs = p.xs + min((tile / n_tiles * CG + (int)rank) * BM + quarter * 32 + lane, p.M - 1);
+      ws = p.ws + (long)(min(tile % n_tiles * BN + c0, p.N - 1) / 128) * KB;
+      x0 = __ldg(xs);
+      w0 = __ldg(ws);
       if (KB > 1) {
         x1 = __ldg(xs + p.M);
         w1 = __ldg(ws + 1);
       }
+    };
+    first_scales(first);
+    for (int tile = first; tile < total && ok; tile += step) {
+      const int mt = tile / n_tiles, nt = tile % n_tiles;
+      const int row0 = (mt * CG + (int)rank) * BM + quarter * 32, n0 = nt * BN + c0;
+      unsigned long long acc[COLS / 2];
+#pragma unroll
+      for (int i = 0; i < COLS / 2; i++) acc[i] = 0;
       for (int kb = 0; kb < KB; kb++, it++) {
         const int a = it % NACC;
         const float sc = x0 * w0;
@@ -281,22 +298,26 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         for (int c = 0; c < COLS; c += 32) {
           uint32_t(&u)[32] = v[(c / 32) & 1];
           wait_ld(u);
-          if (c + 32 < COLS) ld32(t + c + 32, v[(c / 32 + 1) & 1]);
+          if (c + 32 < COLS) {
+            ld32(t + c + 32, v[(c / 32 + 1) & 1]);
+          } else {  // all read: the accumulator is free while the last columns are added
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (CG == 2)
+                mbar_arrive_cluster(map_to_rank(tempty(a), 0));
+              else
+                mbar_arrive(tempty(a));
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 16; i++)
             acc[c / 2 + i] = f2_fma(f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), sc2,
                                     acc[c / 2 + i]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (CG == 2)
-            mbar_arrive_cluster(map_to_rank(tempty(a), 0));
-          else
-            mbar_arrive(tempty(a));
-        }
       }
       if (!ok) break;
+      first_scales(tile + step);  // on their way during the stores
       if (row0 >= p.M) continue;  // warp-uniform
       if (use_tma) {
         constexpr int PER = 128 / sizeof(Y);  // columns of a 128-byte block
@@ -428,16 +449,19 @@ static cudaError_t launch(int ydt, const F8GemmParams& p, DevStatus* status, cud
 }
 
 using Pair = Cfg<2, 256, 5, 2>;
-using Tile128 = Cfg<1, 128, 4, 4>;
-using Tile64 = Cfg<1, 64, 4, 4>;
+using Tile128 = Cfg<1, 128, 5, 4>;
+using Tile64 = Cfg<1, 64, 8, 4>;
 
 template <class Y>
 static cudaError_t pick(int ydt, const F8GemmParams& p, DevStatus* status, cudaStream_t s) {
-  const long mt = (p.M + 127) / 128;
-  // Pairs of 256 x 256 once they fill the 74 pairs of SMs; below that the
-  // widest tile that gives every SM one.
-  if ((mt + 1) / 2 * ((p.N + 255) / 256) >= 74) return launch<Pair, Y>(ydt, p, status, s);
-  if (mt * ((p.N + 127) / 128) >= 148) return launch<Tile128, Y>(ydt, p, status, s);
+  // Measured cost of one wave of tiles, 64 : 128 : 256 wide, about 4 : 5 : 8
+  // (K = 768: 4.1, 5.0 and 6.6 us, K = 4096: 10.4, 13.6 and 20 us).
+  const long sms = 148, m1 = (p.M + 127) / 128, m2 = (m1 + 1) / 2;
+  auto waves = [](long tiles, long slots) { return (tiles + slots - 1) / slots; };
+  const long c64 = 4 * waves(m1 * ((p.N + 63) / 64), sms), c128 = 5 * waves(m1 * ((p.N + 127) / 128), sms),
+             c256 = 8 * waves(m2 * ((p.N + 255) / 256), sms / 2);
+  if (c256 <= c128 && c256 <= c64) return launch<Pair, Y>(ydt, p, status, s);
+  if (c128 <= c64) return launch<Tile128, Y>(ydt, p, status, s);
   return launch<Tile64, Y>(ydt, p, status, s);
 }
 

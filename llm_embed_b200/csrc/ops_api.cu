@@ -230,9 +230,6 @@ int le_f8weight_read(le_f8weight* w, uint8_t* wq, float* scales) {
   return LE_OK;
 }
 
-// Up to this many rows the streaming kernel runs (f8_gemm.cu).
-constexpr int F8_SMALL_MAX_M = 32;
-
 // Quantised activations [M][K], then their scales on a 16-byte boundary.
 static int64_t f8_work_scales_at(int64_t M, int64_t K) { return (M * K + 15) / 16 * 16; }
 
@@ -274,8 +271,10 @@ int le_f8gemm_device(le_f8weight* w, const le_f8gemm_args* a, void* stream) {
   p.ws = w->ws.as<float>();
   p.y = a->y;
   int xt = a->x_type;
+  // Up to F8_FUSED_MAX_M rows are quantised by the product's own kernel; more
+  // are quantised once, before it.
   const bool small = p.M <= F8_SMALL_MAX_M;
-  if (xt != LE_DT_E4M3 && (!small || !aligned(p.x, 16) || (p.ldx * elem_size(xt)) % 16)) {
+  if (xt != LE_DT_E4M3 && (p.M > F8_FUSED_MAX_M || !aligned(p.x, 16) || (p.ldx * elem_size(xt)) % 16)) {
     uint8_t* q = static_cast<uint8_t*>(a->work);
     float* sc = reinterpret_cast<float*>(q + f8_work_scales_at(p.M, p.K));
     CK(launch_f8_quantize(xt, p.x, p.ldx, p.M, p.K, q, sc, s));
