@@ -81,6 +81,12 @@ __device__ __forceinline__ void values8(const Raw8<T>& r, float (&v)[8]) {
     for (int i = 0; i < 4; i++) unpack2(u[i], v[2 * i], v[2 * i + 1], T{});
   }
 }
+// Eight float32 parameters (read-only, 16-byte aligned).
+__device__ __forceinline__ void load_f32x8(const float* p, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
 template <class T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {

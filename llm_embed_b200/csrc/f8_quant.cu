@@ -18,27 +18,24 @@ __device__ __forceinline__ uint32_t group_max(uint32_t a, int width) {
 }
 
 // x [M][K] (row stride ldx) -> q [M][K] bytes, scales [ceil(K/128)][M].
-// Rows 16-byte aligned, K a multiple of 8.  U blocks per lane in flight.
+// Rows 16-byte aligned, K a multiple of 8.  A block has 16 rows, each lane
+// group U consecutive K blocks of one: U loads in flight, and the rows'
+// scales of a K block lie side by side.
 template <class T, int U>
-__global__ void __launch_bounds__(THREADS) quant_vec_kernel(const T* __restrict__ x, long ldx, long items, int M,
-                                                            int K, int KB, uint8_t* __restrict__ q,
+__global__ void __launch_bounds__(THREADS) quant_vec_kernel(const T* __restrict__ x, long ldx, int M, int K, int KB,
+                                                            int steps, uint8_t* __restrict__ q,
                                                             float* __restrict__ scales) {
   pdl_wait();
   pdl_trigger();
-  constexpr int PER = THREADS / G;
   const int lane = threadIdx.x % G;
-  const long item0 = (long)blockIdx.x * (PER * U) + threadIdx.x / G;
+  const long row = (long)(blockIdx.x / steps) * (THREADS / G) + threadIdx.x / G;
+  const int kb0 = blockIdx.x % steps * U;
+  const bool live = row < M;
   Raw8<T> raw[U];
-  long row[U];
-  int kb[U];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const long item = item0 + u * PER;
-    row[u] = items < (1L << 31) ? (long)((uint32_t)item / (uint32_t)KB) : item / KB;
-    kb[u] = (int)(item - row[u] * KB);
-    raw[u] = zero8<T>();
-    const int c = kb[u] * BLOCK + lane * 8;
-    if (item < items && c < K) raw[u] = load8(x + row[u] * ldx + c);
+    const int c = (kb0 + u) * BLOCK + lane * 8;
+    raw[u] = live && c < K ? load8(x + row * ldx + c) : zero8<T>();
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
@@ -50,14 +47,12 @@ __global__ void __launch_bounds__(THREADS) quant_vec_kernel(const T* __restrict_
     a = group_max(a, G);
     float inv;
     const float s = block_scale(a, &inv);
-    const int c = kb[u] * BLOCK + lane * 8;
-    if (item0 + u * PER < items) {
-      if (c < K)
-        *reinterpret_cast<uint2*>(q + row[u] * K + c) =
-            make_uint2(pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                       pack_e4m3(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
-      if (lane == 0) scales[(long)kb[u] * M + row[u]] = s;
-    }
+    const int c = (kb0 + u) * BLOCK + lane * 8;
+    if (live && c < K)
+      *reinterpret_cast<uint2*>(q + row * K + c) =
+          make_uint2(pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                     pack_e4m3(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+    if (live && lane == 0 && kb0 + u < KB) scales[(long)(kb0 + u) * M + row] = s;
   }
 }
 
@@ -126,17 +121,18 @@ static cudaError_t launch(const void* x, long ldx, int M, int K, uint8_t* q, flo
   const long items = (long)M * KB;
   const bool vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * (long)sizeof(T)) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  // Four blocks in flight per lane once that still fills the GPU's 148 SMs.
-  const bool deep = vec && items >= 148L * 4 * 4 * (THREADS / G);
-  const long per = vec ? THREADS / G * (deep ? 4 : 1) : THREADS / 32;
-  const long blocks = (items + per - 1) / per;
+  // Four K blocks in flight per lane once that still gives every one of the
+  // 148 SMs four blocks.
+  const int u = vec && items >= 148L * 4 * 4 * (THREADS / G) ? 4 : 1, steps = (KB + u - 1) / u;
+  const long blocks = vec ? ((long)M + THREADS / G - 1) / (THREADS / G) * steps
+                          : (items + THREADS / 32 - 1) / (THREADS / 32);
   if (blocks > 0x7fffffffL) return cudaErrorInvalidValue;
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)blocks), dim3(THREADS), 0, s, attr);
   const T* xt = static_cast<const T*>(x);
   if (!vec) return cudaLaunchKernelEx(&cfg, quant_any_kernel<T>, xt, ldx, items, M, K, KB, q, scales);
-  if (deep) return cudaLaunchKernelEx(&cfg, quant_vec_kernel<T, 4>, xt, ldx, items, M, K, KB, q, scales);
-  return cudaLaunchKernelEx(&cfg, quant_vec_kernel<T, 1>, xt, ldx, items, M, K, KB, q, scales);
+  if (u == 4) return cudaLaunchKernelEx(&cfg, quant_vec_kernel<T, 4>, xt, ldx, M, K, KB, steps, q, scales);
+  return cudaLaunchKernelEx(&cfg, quant_vec_kernel<T, 1>, xt, ldx, M, K, KB, steps, q, scales);
 }
 
 }  // namespace f8q

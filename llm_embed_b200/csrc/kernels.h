@@ -130,8 +130,9 @@ struct QkNormParams {
   float eps;
   DevStatus* status;
   // set by the launcher
-  int token0;
-  uint32_t items, inv_heads;
+  int token0, q_chunks;
+  uint32_t items, chunks, inv_chunks;
+  float inv_d;
 };
 cudaError_t launch_qk_norm(int dt, QkNormParams p, int n_tokens, cudaStream_t s);
 cudaError_t launch_rope_table(int max_pos, int rot, double base, float* cos, float* sin, cudaStream_t s);
