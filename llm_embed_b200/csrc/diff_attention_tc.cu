@@ -1,0 +1,548 @@
+// Differential attention on the tensor cores (tcgen05, sm_100a), for the
+// sequences that are long enough to fill its tiles:
+//   A_i = softmax(q_i k_i^T / sqrt(d)), o = (A_1 - lambda A_2) v, then the
+//   head's norm (diff_attention.cu has the formulas in full).
+//
+// Persistent kernel, one CTA per SM.  A tile is 128 queries of one head and
+// sequence; its two maps are two chains that share the keys' and values'
+// loads and take turns on the tensor cores: while one map's scores are
+// exponentiated, the other's products run.  A thread of a map's warpgroup has
+// one query row (TMEM lane): it reads the 128 scores of a key block, writes
+// the weights back over them as 16-bit pairs (the A operand of P.V), and keeps
+// the row's maximum and sum.  The maximum that the weights refer to is only
+// moved when it has grown by more than 2^8 (the weights then stay below 2^8,
+// far inside the operand's range, and the sums are float32), so rescaling the
+// result in TMEM is rare.  Bound by the exponentials: two per query, key and
+// head, 16 a clock and SM.
+//
+//   warp 0      producer: TMA loads of Q (two stages), K and V (two each)
+//   warp 1      TMEM allocation; MMAs: S_i = Q_i K_i^T, O_i += P_i V
+//   warp 3      finds the tiles' sequences and publishes them in a ring
+//   warps 4-7   map 1, warps 8-11 map 2: softmax; then each group combines
+//               half of the columns of O_1 and O_2, norms and stores them
+// TMEM (512 columns): S_1 / P_1, S_2 / P_2 (128 each), O_1, O_2 (2d each).
+// A map's MMAs run in the order they are issued, so S_i of the next block may
+// overwrite P_i once P_i.V is issued, and a row that sees S_i of block j
+// complete also sees O_i of block j - 1 complete.
+//
+// Keys past the sequence: their scores count as -inf; P.V stops at the next
+// multiple of 16 keys, and the values between (another sequence's, or
+// garbage) are overwritten with zeros in shared memory before it, so nothing
+// but the sequence's own rows reaches a result.  Query rows past it are not
+// stored.  Every mbarrier wait is bounded (WAIT_LIMIT_NS).
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "diff_attention.cuh"
+#include "gemm_epi_tc.cuh"
+#include "softmax_tc.cuh"
+#include "tcgen05.cuh"
+
+namespace le {
+namespace dtc {
+
+using namespace tcx;
+using namespace dif;
+
+constexpr int BQ = 128, BKEY = 128;
+constexpr int TILE = 128 * 128;  // bytes of 128 rows x 64 columns
+constexpr int NTHREADS = 384;
+constexpr int RING = 3;
+constexpr float GROW = 8.f;  // log2 of the growth that moves the maximum
+
+template <int D>
+struct Lay {
+  static constexpr int NT = 2 * D / 64;   // 64-column tiles of an operand
+  static constexpr int OP = NT * TILE;    // bytes of 128 rows of Q, K or V
+  static constexpr int OFF_Q = 0;         // [2]
+  static constexpr int OFF_K = 2 * OP;    // [2]
+  static constexpr int OFF_V = 4 * OP;    // [2]
+  static constexpr int OFF_L = 6 * OP;    // sums [2 tiles][2 maps][128], squares likewise
+  static constexpr int OFF_RING = OFF_L + 2 * 2 * 2 * 128 * 4;
+  static constexpr int OFF_BAR = OFF_RING + RING * 16;
+  // q_full q_empty k_full k_empty v_full v_empty [2 each], s_full p_full [2],
+  // o_full o_empty, ring_full ring_empty [RING], sum_full sq_full
+  static constexpr int NBAR = 12 + 4 + 2 + 2 * RING + 2;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int ALLOC = OFF_MISC + 16 + 1024;
+  static_assert(ALLOC <= 232448, "shared memory of one CTA");
+};
+
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%"
+      "20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// D (TMEM) (+)= A (TMEM: lane = row, two 16-bit values of K per column) . B.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+  return e != 0;
+}
+// 32 bytes of a row.
+__device__ __forceinline__ void store32(void* p, const uint32_t* w, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    static_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(NTHREADS, 1)
+    diff_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                   const __grid_constant__ CUtensorMap tmap_v, DiffParams p, int tiles, int wide) {
+  using L = Lay<D>;
+  constexpr int NT = L::NT, OP = L::OP, W = 2 * D;
+  constexpr uint32_t FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0;
+  constexpr uint32_t IDESC_S = idesc_f16(BQ, BKEY) | FMT;
+  constexpr uint32_t IDESC_O = idesc_f16(BQ, W) | FMT | (1u << 16);  // B (V) MN-major
+  constexpr uint32_t TM_O = 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t sbase = smem_u32(smem), bar0 = sbase + L::OFF_BAR;
+  auto q_full = [&](int s) { return bar0 + 8 * s; };
+  auto q_empty = [&](int s) { return bar0 + 8 * (2 + s); };
+  auto k_full = [&](int s) { return bar0 + 8 * (4 + s); };
+  auto k_empty = [&](int s) { return bar0 + 8 * (6 + s); };
+  auto v_full = [&](int s) { return bar0 + 8 * (8 + s); };
+  auto v_empty = [&](int s) { return bar0 + 8 * (10 + s); };
+  auto s_full = [&](int i) { return bar0 + 8 * (12 + i); };
+  auto p_full = [&](int i) { return bar0 + 8 * (14 + i); };
+  const uint32_t o_full = bar0 + 8 * 16, o_empty = bar0 + 8 * 17;
+  auto ring_full = [&](int e) { return bar0 + 8 * (18 + e); };
+  auto ring_empty = [&](int e) { return bar0 + 8 * (18 + RING + e); };
+  const uint32_t sum_full = bar0 + 8 * (18 + 2 * RING), sq_full = sum_full + 8;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC + 4);
+  int4* ring = reinterpret_cast<int4*>(smem + L::OFF_RING);  // {t0, len, q0, head}, len 0: no more
+  DevStatus* status = p.status;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < 16; i++) mbar_init(bar0 + 8 * i, i >= 14 ? 4 : 1);  // p_full: the map's four warps
+    mbar_init(o_full, 1);
+    mbar_init(o_empty, 8);
+    mbar_init(sum_full, 8);
+    mbar_init(sq_full, 8);
+    for (int e = 0; e < RING; e++) {
+      mbar_init(ring_full(e), 1);
+      mbar_init(ring_empty(e), 10);  // producer, MMA, eight softmax warps
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  // The next tile of the ring, for a whole warp; false at the end.
+  auto next_tile = [&](uint32_t n, int4& tile) -> bool {
+    const int e = n % RING;
+    if (!__all_sync(0xffffffffu, mbar_wait(ring_full(e), (n / RING) & 1, abort_flag, status, 60))) return false;
+    tile = ring[e];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(ring_empty(e));
+    return tile.y > 0;
+  };
+
+  // 384 threads of 168 registers at launch: the softmax threads hold 128
+  // scores each.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 3) {
+      // -------------------------------------------------------------- tiles
+      if (blockIdx.x == 0) check_offsets(p, 32);
+      uint32_t n = 0;
+      auto publish = [&](int4 t) -> bool {
+        const int e = n % RING;
+        if (!__all_sync(0xffffffffu, mbar_wait(ring_empty(e), ((n / RING) & 1) ^ 1, abort_flag, status, 61)))
+          return false;
+        if (lane == 0) {
+          ring[e] = t;
+          mbar_arrive(ring_full(e));
+        }
+        n++;
+        return true;
+      };
+      Where w{};
+      int last = -1;
+      bool found = false, ok = true;
+      const long items = (long)tiles * p.heads;
+      for (long item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        const int tile = (int)(item / p.heads), head = (int)(item - (long)tile * p.heads);
+        if (tile != last) found = find_block(p, tile, BQ, w) && w.len >= p.min_len;
+        last = tile;
+        if (found) ok = publish(make_int4(w.t0, w.len, w.q0, head));
+      }
+      if (ok) publish(make_int4(0, 0, 0, 0));
+    } else if (warp == 0) {
+      // ----------------------------------------------------------- producer
+      const bool issuer = elect_one();
+      uint32_t n = 0, ib = 0;  // tiles, key blocks
+      int4 t;
+      bool ok = true;
+      auto load = [&](const CUtensorMap* map, uint32_t dst, int col, int row, uint32_t bar) {
+        mbar_expect_tx(bar, OP);
+#pragma unroll
+        for (int c = 0; c < NT; c++) tma_load_2d(dst + c * TILE, map, col + c * 64, row, bar);
+      };
+      while (ok && next_tile(n, t)) {
+        const int qs = n & 1, kcol = t.w / p.group * W, nkb = (t.y + BKEY - 1) / BKEY;
+        ok = __all_sync(0xffffffffu, mbar_wait(q_empty(qs), ((n >> 1) & 1) ^ 1, abort_flag, status, 62));
+        if (!ok) break;
+        if (issuer) load(&tmap_q, sbase + L::OFF_Q + qs * OP, t.w * W, t.x + t.z, q_full(qs));
+        for (int j = 0; j < nkb && ok; j++, ib++) {
+          const int s = ib & 1, row = t.x + j * BKEY;
+          const uint32_t ph = ((ib >> 1) & 1) ^ 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(k_empty(s), ph, abort_flag, status, 63));
+          if (!ok) break;
+          if (issuer) load(&tmap_k, sbase + L::OFF_K + s * OP, kcol, row, k_full(s));
+          ok = __all_sync(0xffffffffu, mbar_wait(v_empty(s), ph, abort_flag, status, 64));
+          if (!ok) break;
+          if (issuer) load(&tmap_v, sbase + L::OFF_V + s * OP, kcol, row, v_full(s));
+        }
+        n++;
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA
+      const bool issuer = elect_one();
+      uint32_t n = 0, ib = 0;
+      int4 t;
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, site));
+        return ok;
+      };
+      while (ok && next_tile(n, t)) {
+        const int qs = n & 1, nkb = (t.y + BKEY - 1) / BKEY;
+        // Map i of an operand with d = 64 is a tile of its own, with d = 32
+        // half of the 128-byte rows.
+        auto map_off = [](int i) { return D == 64 ? i * TILE : i * 64; };
+        auto issue_s = [&](int i, uint32_t b) {  // S_i of block number b
+          if (issuer) {
+            const uint64_t qd = sw128_desc(sbase + L::OFF_Q + qs * OP + map_off(i));
+            const uint64_t kd = sw128_desc(sbase + L::OFF_K + (b & 1) * OP + map_off(i));
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk++) mma_f16(tmem + i * 128, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk != 0);
+            mma_commit(s_full(i));
+          }
+          __syncwarp();
+        };
+        auto issue_pv = [&](int i, uint32_t b, int steps, bool first) {
+          if (issuer) {
+            // V [keys][64] tiles side by side: TILE bytes from one 64-column
+            // group to the next (leading offset), 16 keys = 2048 bytes.
+            const uint64_t vd = (sw128_desc(sbase + L::OFF_V + (b & 1) * OP) & ~((uint64_t)0x3FFF << 16)) |
+                                ((uint64_t)(TILE >> 4) << 16);
+#pragma unroll
+            for (int kk = 0; kk < BKEY / 16; kk++)
+              if (kk < steps)
+                mma_ts(tmem + TM_O + i * W, tmem + i * 128 + kk * 8, vd + kk * (2048 >> 4), IDESC_O,
+                       !(first && kk == 0));
+          }
+          __syncwarp();
+        };
+        if (!wait(q_full(qs), (n >> 1) & 1, 65) || !wait(k_full(ib & 1), (ib >> 1) & 1, 66)) break;
+        tc_fence_after();
+        issue_s(0, ib);
+        issue_s(1, ib);
+        if (issuer) {
+          mma_commit(k_empty(ib & 1));
+          if (nkb == 1) mma_commit(q_empty(qs));
+        }
+        __syncwarp();
+        for (int j = 0; j < nkb; j++, ib++) {
+          const int steps = min(BKEY, t.y - j * BKEY + 15) / 16;
+          const uint32_t ph = (ib >> 1) & 1, nb = ib + 1;
+          if (!wait(v_full(ib & 1), ph, 67) || (j == 0 && !wait(o_empty, (n & 1) ^ 1, 68)) ||
+              !wait(p_full(0), ib & 1, 69))
+            break;
+          tc_fence_after();
+          issue_pv(0, ib, steps, j == 0);
+          if (j + 1 < nkb) {
+            if (!wait(k_full(nb & 1), (nb >> 1) & 1, 72)) break;
+            tc_fence_after();
+            issue_s(0, nb);
+          }
+          if (!wait(p_full(1), ib & 1, 73)) break;
+          tc_fence_after();
+          issue_pv(1, ib, steps, j == 0);
+          if (issuer) mma_commit(v_empty(ib & 1));
+          __syncwarp();
+          if (j + 1 < nkb) {
+            issue_s(1, nb);
+            if (issuer) {
+              mma_commit(k_empty(nb & 1));
+              if (j + 2 == nkb) mma_commit(q_empty(qs));
+            }
+            __syncwarp();
+          }
+        }
+        if (!ok) break;
+        if (issuer) mma_commit(o_full);
+        __syncwarp();
+        n++;
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // -------------------------------------------------------------- softmax
+    const int map = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t ts = tmem + map * 128 + lanes, to = tmem + TM_O + map * W + lanes;
+    const float scale = 1.4426950408889634f * rsqrtf((float)D);
+    const unsigned long long scale2 = f2_pack(scale, scale);
+    float* sums = reinterpret_cast<float*>(smem + L::OFF_L);
+    uint32_t n = 0, ib = 0;
+    int4 t;
+    bool ok = true;
+    while (ok && next_tile(n, t)) {
+      const int nkb = (t.y + BKEY - 1) / BKEY;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nkb; j++, ib++) {
+        ok = __all_sync(0xffffffffu, mbar_wait(s_full(map), ib & 1, abort_flag, status, 74));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t r[128];
+#pragma unroll
+        for (int c = 0; c < 4; c++) ld32(ts + 32 * c, r + 32 * c);
+        wait_ld();
+        const int left = t.y - j * BKEY;  // keys of this block and behind
+        if (left < BKEY) {
+#pragma unroll
+          for (int e = 0; e < 128; e++) r[e] = e < left ? r[e] : 0xff800000u;
+        }
+        float m0 = m, m1 = -INFINITY;
+        chunk_max<128>(m0, m1, r, 128);
+        m0 = fmaxf(m0, m1);
+        if (j == 0) {
+          m = m0;
+        } else if (__any_sync(0xffffffffu, (m0 - m) * scale > GROW)) {
+          const float f = ex2((m - m0) * scale);
+          const unsigned long long f2 = f2_pack(f, f);
+          m = m0;
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < W; c += 16) {
+            float v[16];
+            uint32_t w[16];
+            tmem_ld16(to + c, v);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              float a, b;
+              f2_unpack(f2_mul(f2_pack(v[e], v[e + 1]), f2), a, b);
+              w[e] = __float_as_uint(a);
+              w[e + 1] = __float_as_uint(b);
+            }
+            st16(to + c, w);
+          }
+        }
+        const unsigned long long off = f2_pack(-m * scale, -m * scale);
+        unsigned long long s0 = 0, s1 = 0;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            float x0, x1;
+            const int at = 32 * c + 2 * e;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(r[at]), __uint_as_float(r[at + 1])), scale2, off), x0, x1);
+            x0 = ex2(x0);
+            x1 = ex2(x1);
+            if (e & 1)
+              s1 = f2_add(s1, f2_pack(x0, x1));
+            else
+              s0 = f2_add(s0, f2_pack(x0, x1));
+            w[e] = pack2<T>(x0, x1);
+          }
+          st16(ts + 16 * c, w);
+        }
+        float a, b;
+        f2_unpack(f2_add(s0, s1), a, b);
+        l += a + b;
+        if (map == 0 && left < BKEY && left % 16 != 0) {
+          // The values between the last key and the end of its 16.
+          ok = __all_sync(0xffffffffu, mbar_wait(v_full(ib & 1), (ib >> 1) & 1, abort_flag, status, 75));
+          if (!ok) break;
+          const int rows = 16 - left % 16;
+          uint8_t* v = smem + L::OFF_V + (ib & 1) * OP + left * 128;
+          for (int e = row; e < rows * 8 * NT; e += 128)
+            *reinterpret_cast<uint4*>(v + e / (rows * 8) * TILE + e % (rows * 8) * 16) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(map));
+      }
+      if (!ok) break;
+      // ------------------------------------------------------------ result
+      // The groups exchange their rows' sums (two buffers: a group may be at
+      // the next tile's before the other has read these) and take half of the
+      // columns each.
+      float* sum = sums + (n & 1) * 256;
+      float* sq = sums + 512 + (n & 1) * 256;
+      // Eight warps meet at a barrier whose wait is bounded as all others.
+      auto meet = [&](uint32_t bar, int site) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+        return __all_sync(0xffffffffu, mbar_wait(bar, n & 1, abort_flag, status, site)) != 0;
+      };
+      sum[map * 128 + row] = l;
+      ok = meet(sum_full, 77) && __all_sync(0xffffffffu, mbar_wait(o_full, n & 1, abort_flag, status, 76));
+      if (!ok) break;
+      tc_fence_after();
+      const float w1 = 1.f / sum[row], w2 = p.lambda[t.w] / sum[128 + row];
+      const uint32_t o1 = tmem + TM_O + lanes + map * D, o2 = o1 + W;
+      float o[D], ss = 0.f;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t a[32], b[32];
+        ld32(o1 + c, a);
+        ld32(o2 + c, b);
+        wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e++) {
+          o[c + e] = fmaf(__uint_as_float(a[e]), w1, -__uint_as_float(b[e]) * w2);
+          ss = fmaf(o[c + e], o[c + e], ss);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_empty);
+      const float* nw = p.norm_w;
+      if (nw) {
+        sq[map * 128 + row] = ss;
+        ok = meet(sq_full, 78);
+        if (!ok) break;
+        const float f = p.out_scale * rsqrtf((sq[row] + sq[128 + row]) / (float)W + p.eps);
+#pragma unroll
+        for (int c = 0; c < D; c += 8) {
+          float w[8];
+          load_f32x8(nw + map * D + c, w);
+#pragma unroll
+          for (int e = 0; e < 8; e++) o[c + e] *= f * w[e];
+        }
+      }
+      if (t.z + row < t.y) {
+        T* out = static_cast<T*>(p.out) + (long)(t.x + t.z + row) * p.o_stride + (long)t.w * W + map * D;
+#pragma unroll
+        for (int c = 0; c < D; c += 16) {
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) w[e] = pack2<T>(o[c + 2 * e], o[c + 2 * e + 1]);
+          store32(out + c, w, wide);
+        }
+      }
+      n++;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// ---------------------------------------------------------------- host ----
+
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+template <class T, int D>
+static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
+  auto enc = encode_fn();
+  if (!enc) return cudaErrorNotSupported;
+  auto encode = [&](CUtensorMap* map, const void* ptr, int heads, long ld) {
+    const cuuint64_t dims[2] = {(cuuint64_t)heads * 2 * D, (cuuint64_t)p.T};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {64, 128};
+    const cuuint32_t estr[2] = {1, 1};
+    const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return enc(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  CUtensorMap mq, mk, mv;
+  const int kvh = p.heads / p.group;
+  if (!encode(&mq, p.q, p.heads, p.q_stride) || !encode(&mk, p.k, kvh, p.k_stride) || !encode(&mv, p.v, kvh, p.v_stride))
+    return cudaErrorInvalidValue;
+  static std::mutex mu;
+  static int sms[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64) return cudaErrorInvalidDevice;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (sms[dev] == 0) {
+      cudaError_t e =
+          cudaFuncSetAttribute(diff_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::ALLOC);
+      if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+      if (e != cudaSuccess) return e;
+    }
+  }
+  const int tiles = block_count(p.T, p.nseq, BQ);
+  const long items = (long)tiles * p.heads;
+  const int wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.o_stride % 16 == 0;
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)(items < sms[dev] ? items : sms[dev])), dim3(NTHREADS),
+                                            Lay<D>::ALLOC, s, attr);
+  return cudaLaunchKernelEx(&cfg, diff_tc_kernel<T, D>, mq, mk, mv, p, tiles, wide);
+}
+
+}  // namespace dtc
+
+cudaError_t launch_diff_attention_tc(int dt, int d, const DiffParams& p, cudaStream_t s) {
+  if (p.nseq == 0 || p.T == 0) return cudaSuccess;
+  if (dt == DT_F16) return d == 64 ? dtc::launch<__half, 64>(p, s) : dtc::launch<__half, 32>(p, s);
+  return d == 64 ? dtc::launch<__nv_bfloat16, 64>(p, s) : dtc::launch<__nv_bfloat16, 32>(p, s);
+}
+
+}  // namespace le

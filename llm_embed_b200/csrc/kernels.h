@@ -169,8 +169,11 @@ struct DiffParams {
   const float* lambda;     // [heads]
   const float* norm_w;     // [2d] or null
   float out_scale, eps;    // 1 - lambda_init
+  int min_len, max_len;    // the launch's sequences: others are left to another
   DevStatus* status;
 };
 cudaError_t launch_diff_attention(int dt, int d, const DiffParams& p, cudaStream_t s);
+// diff_attention_tc.cu: the same on tcgen05 tiles of 128 queries and keys.
+cudaError_t launch_diff_attention_tc(int dt, int d, const DiffParams& p, cudaStream_t s);
 
 }  // namespace le

@@ -450,7 +450,14 @@ int le_diffattn_device(le_diffattn* h, const le_diffattn_args* a, void* stream) 
   p.status = h->st();
   DeviceGuard g(h->dev);
   CK(g.err);
-  CK(launch_diff_attention(a->type, h->d, p, h->pick(stream)));
+  const cudaStream_t s = h->pick(stream);
+  const int path = getenv("LE_DIFF") ? atoi(getenv("LE_DIFF")) : 1;
+  p.min_len = 0;
+  p.max_len = 0x7fffffff;
+  if (path == 1)
+    CK(launch_diff_attention_tc(a->type, h->d, p, s));
+  else
+    CK(launch_diff_attention(a->type, h->d, p, s));
   return LE_OK;
 }
 
