@@ -7,7 +7,7 @@
 // sequence; its two maps are two chains that share the keys' and values'
 // loads and take turns on the tensor cores: while one map's scores are
 // exponentiated, the other's products run.  A thread of a map's warpgroup has
-// one query row (TMEM lane): it reads the 128 scores of a key block, writes
+// one query row (TMEM lane): it reads the 64 scores of a key block, writes
 // the weights back over them as 16-bit pairs (the A operand of P.V), and keeps
 // the row's maximum and sum.  The maximum that the weights refer to is only
 // moved when it has grown by more than 2^8 (the weights then stay below 2^8,
@@ -15,15 +15,15 @@
 // result in TMEM is rare.  Bound by the exponentials: two per query, key and
 // head, 16 a clock and SM.
 //
-//   warp 0      producer: TMA loads of Q (two stages), K and V (two each)
+//   warp 0      producer: TMA loads of Q (two stages), K and V (four each)
 //   warp 1      TMEM allocation; MMAs: S_i = Q_i K_i^T, O_i += P_i V
 //   warp 3      finds the tiles' sequences and publishes them in a ring
 //   warps 4-7   map 1, warps 8-11 map 2: softmax; then each group combines
 //               half of the columns of O_1 and O_2, norms and stores them
-// TMEM (512 columns): S_1 / P_1, S_2 / P_2 (128 each), O_1, O_2 (2d each).
-// A map's MMAs run in the order they are issued, so S_i of the next block may
-// overwrite P_i once P_i.V is issued, and a row that sees S_i of block j
-// complete also sees O_i of block j - 1 complete.
+// TMEM (512 columns): two buffers of S_i / P_i for each map (64 each), O_1,
+// O_2 (2d each).  A map's MMAs run in the order they are issued - S of block
+// j + 2 after P.V of block j, whose buffer it takes - so a map has a block of
+// scores waiting while another's weights are multiplied.
 //
 // Keys past the sequence: their scores count as -inf; P.V stops at the next
 // multiple of 16 keys, and the values between (another sequence's, or
@@ -45,8 +45,9 @@ namespace dtc {
 using namespace tcx;
 using namespace dif;
 
-constexpr int BQ = 128, BKEY = 128;
-constexpr int TILE = 128 * 128;  // bytes of 128 rows x 64 columns
+constexpr int BQ = 128, BKEY = 64;
+constexpr int QTILE = 128 * 128, KTILE = 64 * 128;  // bytes of 128 and 64 rows x 64 columns
+constexpr int KV = 4;                               // stages of K and of V
 constexpr int NTHREADS = 384;
 constexpr int RING = 3;
 constexpr float GROW = 8.f;  // log2 of the growth that moves the maximum
@@ -54,16 +55,19 @@ constexpr float GROW = 8.f;  // log2 of the growth that moves the maximum
 template <int D>
 struct Lay {
   static constexpr int NT = 2 * D / 64;   // 64-column tiles of an operand
-  static constexpr int OP = NT * TILE;    // bytes of 128 rows of Q, K or V
+  static constexpr int QB = NT * QTILE;   // bytes of a query tile
+  static constexpr int KB = NT * KTILE;   // bytes of a block of K or V
   static constexpr int OFF_Q = 0;         // [2]
-  static constexpr int OFF_K = 2 * OP;    // [2]
-  static constexpr int OFF_V = 4 * OP;    // [2]
-  static constexpr int OFF_L = 6 * OP;    // sums [2 tiles][2 maps][128], squares likewise
+  static constexpr int OFF_K = 2 * QB;    // [KV]
+  static constexpr int OFF_V = OFF_K + KV * KB;  // [KV]
+  static constexpr int OFF_L = OFF_V + KV * KB;  // sums [2 tiles][2 maps][128], squares likewise
   static constexpr int OFF_RING = OFF_L + 2 * 2 * 2 * 128 * 4;
   static constexpr int OFF_BAR = OFF_RING + RING * 16;
-  // q_full q_empty k_full k_empty v_full v_empty [2 each], s_full p_full [2],
-  // o_full o_empty, ring_full ring_empty [RING], sum_full sq_full
-  static constexpr int NBAR = 12 + 4 + 2 + 2 * RING + 2;
+  // q_full q_empty [2 each], k_full k_empty v_full v_empty [KV each], s_full
+  // p_full [2 maps][2], o_done [2], o_full o_empty sum_full sq_full, ring_full
+  // ring_empty [RING]
+  static constexpr int B_Q = 0, B_K = 4, B_V = B_K + 2 * KV, B_S = B_V + 2 * KV, B_P = B_S + 4, B_D = B_P + 4,
+                       B_O = B_D + 2, B_R = B_O + 4, NBAR = B_R + 2 * RING;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;
   static_assert(ALLOC <= 232448, "shared memory of one CTA");
@@ -118,7 +122,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     diff_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                    const __grid_constant__ CUtensorMap tmap_v, DiffParams p, int tiles, int wide) {
   using L = Lay<D>;
-  constexpr int NT = L::NT, OP = L::OP, W = 2 * D;
+  constexpr int NT = L::NT, W = 2 * D;
   constexpr uint32_t FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0;
   constexpr uint32_t IDESC_S = idesc_f16(BQ, BKEY) | FMT;
   constexpr uint32_t IDESC_O = idesc_f16(BQ, W) | FMT | (1u << 16);  // B (V) MN-major
@@ -126,18 +130,18 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = smem_u32(smem), bar0 = sbase + L::OFF_BAR;
-  auto q_full = [&](int s) { return bar0 + 8 * s; };
-  auto q_empty = [&](int s) { return bar0 + 8 * (2 + s); };
-  auto k_full = [&](int s) { return bar0 + 8 * (4 + s); };
-  auto k_empty = [&](int s) { return bar0 + 8 * (6 + s); };
-  auto v_full = [&](int s) { return bar0 + 8 * (8 + s); };
-  auto v_empty = [&](int s) { return bar0 + 8 * (10 + s); };
-  auto s_full = [&](int i) { return bar0 + 8 * (12 + i); };
-  auto p_full = [&](int i) { return bar0 + 8 * (14 + i); };
-  const uint32_t o_full = bar0 + 8 * 16, o_empty = bar0 + 8 * 17;
-  auto ring_full = [&](int e) { return bar0 + 8 * (18 + e); };
-  auto ring_empty = [&](int e) { return bar0 + 8 * (18 + RING + e); };
-  const uint32_t sum_full = bar0 + 8 * (18 + 2 * RING), sq_full = sum_full + 8;
+  auto q_full = [&](int s) { return bar0 + 8 * (L::B_Q + s); };
+  auto q_empty = [&](int s) { return bar0 + 8 * (L::B_Q + 2 + s); };
+  auto k_full = [&](int s) { return bar0 + 8 * (L::B_K + s); };
+  auto k_empty = [&](int s) { return bar0 + 8 * (L::B_K + KV + s); };
+  auto v_full = [&](int s) { return bar0 + 8 * (L::B_V + s); };
+  auto v_empty = [&](int s) { return bar0 + 8 * (L::B_V + KV + s); };
+  auto s_full = [&](int i, uint32_t b) { return bar0 + 8 * (L::B_S + 2 * i + (b & 1)); };
+  auto p_full = [&](int i, uint32_t b) { return bar0 + 8 * (L::B_P + 2 * i + (b & 1)); };
+  auto o_done = [&](int i) { return bar0 + 8 * (L::B_D + i); };
+  const uint32_t o_full = bar0 + 8 * L::B_O, o_empty = o_full + 8, sum_full = o_full + 16, sq_full = o_full + 24;
+  auto ring_full = [&](int e) { return bar0 + 8 * (L::B_R + e); };
+  auto ring_empty = [&](int e) { return bar0 + 8 * (L::B_R + RING + e); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC + 4);
   int4* ring = reinterpret_cast<int4*>(smem + L::OFF_RING);  // {t0, len, q0, head}, len 0: no more
@@ -146,8 +150,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int i = 0; i < 16; i++) mbar_init(bar0 + 8 * i, i >= 14 ? 4 : 1);  // p_full: the map's four warps
-    mbar_init(o_full, 1);
+    for (int i = 0; i <= L::B_O; i++) mbar_init(bar0 + 8 * i, i >= L::B_P && i < L::B_D ? 4 : 1);  // p_full: four warps
     mbar_init(o_empty, 8);
     mbar_init(sum_full, 8);
     mbar_init(sq_full, 8);
@@ -215,25 +218,25 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       uint32_t n = 0, ib = 0;  // tiles, key blocks
       int4 t;
       bool ok = true;
-      auto load = [&](const CUtensorMap* map, uint32_t dst, int col, int row, uint32_t bar) {
-        mbar_expect_tx(bar, OP);
+      auto load = [&](const CUtensorMap* map, uint32_t dst, int bytes, int col, int row, uint32_t bar) {
+        mbar_expect_tx(bar, NT * bytes);
 #pragma unroll
-        for (int c = 0; c < NT; c++) tma_load_2d(dst + c * TILE, map, col + c * 64, row, bar);
+        for (int c = 0; c < NT; c++) tma_load_2d(dst + c * bytes, map, col + c * 64, row, bar);
       };
       while (ok && next_tile(n, t)) {
         const int qs = n & 1, kcol = t.w / p.group * W, nkb = (t.y + BKEY - 1) / BKEY;
         ok = __all_sync(0xffffffffu, mbar_wait(q_empty(qs), ((n >> 1) & 1) ^ 1, abort_flag, status, 62));
         if (!ok) break;
-        if (issuer) load(&tmap_q, sbase + L::OFF_Q + qs * OP, t.w * W, t.x + t.z, q_full(qs));
+        if (issuer) load(&tmap_q, sbase + L::OFF_Q + qs * L::QB, QTILE, t.w * W, t.x + t.z, q_full(qs));
         for (int j = 0; j < nkb && ok; j++, ib++) {
-          const int s = ib & 1, row = t.x + j * BKEY;
-          const uint32_t ph = ((ib >> 1) & 1) ^ 1;
+          const int s = ib % KV, row = t.x + j * BKEY;
+          const uint32_t ph = ((ib / KV) & 1) ^ 1;
           ok = __all_sync(0xffffffffu, mbar_wait(k_empty(s), ph, abort_flag, status, 63));
           if (!ok) break;
-          if (issuer) load(&tmap_k, sbase + L::OFF_K + s * OP, kcol, row, k_full(s));
+          if (issuer) load(&tmap_k, sbase + L::OFF_K + s * L::KB, KTILE, kcol, row, k_full(s));
           ok = __all_sync(0xffffffffu, mbar_wait(v_empty(s), ph, abort_flag, status, 64));
           if (!ok) break;
-          if (issuer) load(&tmap_v, sbase + L::OFF_V + s * OP, kcol, row, v_full(s));
+          if (issuer) load(&tmap_v, sbase + L::OFF_V + s * L::KB, KTILE, kcol, row, v_full(s));
         }
         n++;
       }
@@ -251,65 +254,74 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         const int qs = n & 1, nkb = (t.y + BKEY - 1) / BKEY;
         // Map i of an operand with d = 64 is a tile of its own, with d = 32
         // half of the 128-byte rows.
-        auto map_off = [](int i) { return D == 64 ? i * TILE : i * 64; };
         auto issue_s = [&](int i, uint32_t b) {  // S_i of block number b
           if (issuer) {
-            const uint64_t qd = sw128_desc(sbase + L::OFF_Q + qs * OP + map_off(i));
-            const uint64_t kd = sw128_desc(sbase + L::OFF_K + (b & 1) * OP + map_off(i));
+            const uint64_t qd = sw128_desc(sbase + L::OFF_Q + qs * L::QB + i * (D == 64 ? QTILE : 64));
+            const uint64_t kd = sw128_desc(sbase + L::OFF_K + (b % KV) * L::KB + i * (D == 64 ? KTILE : 64));
 #pragma unroll
-            for (int kk = 0; kk < D / 16; kk++) mma_f16(tmem + i * 128, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk != 0);
-            mma_commit(s_full(i));
+            for (int kk = 0; kk < D / 16; kk++)
+              mma_f16(tmem + i * 128 + (b & 1) * BKEY, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk != 0);
+            mma_commit(s_full(i, b));
           }
           __syncwarp();
         };
         auto issue_pv = [&](int i, uint32_t b, int steps, bool first) {
           if (issuer) {
-            // V [keys][64] tiles side by side: TILE bytes from one 64-column
+            // V [keys][64] tiles side by side: KTILE bytes from one 64-column
             // group to the next (leading offset), 16 keys = 2048 bytes.
-            const uint64_t vd = (sw128_desc(sbase + L::OFF_V + (b & 1) * OP) & ~((uint64_t)0x3FFF << 16)) |
-                                ((uint64_t)(TILE >> 4) << 16);
+            const uint64_t vd = (sw128_desc(sbase + L::OFF_V + (b % KV) * L::KB) & ~((uint64_t)0x3FFF << 16)) |
+                                ((uint64_t)(KTILE >> 4) << 16);
 #pragma unroll
             for (int kk = 0; kk < BKEY / 16; kk++)
               if (kk < steps)
-                mma_ts(tmem + TM_O + i * W, tmem + i * 128 + kk * 8, vd + kk * (2048 >> 4), IDESC_O,
+                mma_ts(tmem + TM_O + i * W, tmem + i * 128 + (b & 1) * BKEY + kk * 8, vd + kk * (2048 >> 4), IDESC_O,
                        !(first && kk == 0));
+            mma_commit(o_done(i));
           }
           __syncwarp();
         };
-        if (!wait(q_full(qs), (n >> 1) & 1, 65) || !wait(k_full(ib & 1), (ib >> 1) & 1, 66)) break;
-        tc_fence_after();
-        issue_s(0, ib);
-        issue_s(1, ib);
-        if (issuer) {
-          mma_commit(k_empty(ib & 1));
-          if (nkb == 1) mma_commit(q_empty(qs));
-        }
-        __syncwarp();
+        auto k_ready = [&](uint32_t b) {
+          if (!wait(k_full(b % KV), (b / KV) & 1, 66)) return false;
+          tc_fence_after();
+          return true;
+        };
+        // K of block b is read; Q too with the tile's last.
+        auto k_done = [&](uint32_t b, bool last) {
+          if (issuer) {
+            mma_commit(k_empty(b % KV));
+            if (last) mma_commit(q_empty(qs));
+          }
+          __syncwarp();
+        };
+        if (!wait(q_full(qs), (n >> 1) & 1, 65)) break;
+        // The scores run two blocks ahead of the values.
+        for (int j = 0; j < 2 && j < nkb && ok; j++)
+          if (k_ready(ib + j)) {
+            issue_s(0, ib + j);
+            issue_s(1, ib + j);
+            k_done(ib + j, j + 1 == nkb);
+          }
+        if (!ok) break;
         for (int j = 0; j < nkb; j++, ib++) {
           const int steps = min(BKEY, t.y - j * BKEY + 15) / 16;
-          const uint32_t ph = (ib >> 1) & 1, nb = ib + 1;
-          if (!wait(v_full(ib & 1), ph, 67) || (j == 0 && !wait(o_empty, (n & 1) ^ 1, 68)) ||
-              !wait(p_full(0), ib & 1, 69))
+          const bool more = j + 2 < nkb;
+          if (!wait(v_full(ib % KV), (ib / KV) & 1, 67) || (j == 0 && !wait(o_empty, (n & 1) ^ 1, 68)) ||
+              !wait(p_full(0, ib), (ib >> 1) & 1, 69))
             break;
           tc_fence_after();
           issue_pv(0, ib, steps, j == 0);
-          if (j + 1 < nkb) {
-            if (!wait(k_full(nb & 1), (nb >> 1) & 1, 72)) break;
-            tc_fence_after();
-            issue_s(0, nb);
+          if (more) {
+            if (!k_ready(ib + 2)) break;
+            issue_s(0, ib + 2);
           }
-          if (!wait(p_full(1), ib & 1, 73)) break;
+          if (!wait(p_full(1, ib), (ib >> 1) & 1, 73)) break;
           tc_fence_after();
           issue_pv(1, ib, steps, j == 0);
-          if (issuer) mma_commit(v_empty(ib & 1));
+          if (issuer) mma_commit(v_empty(ib % KV));
           __syncwarp();
-          if (j + 1 < nkb) {
-            issue_s(1, nb);
-            if (issuer) {
-              mma_commit(k_empty(nb & 1));
-              if (j + 2 == nkb) mma_commit(q_empty(qs));
-            }
-            __syncwarp();
+          if (more) {
+            issue_s(1, ib + 2);
+            k_done(ib + 2, j + 3 == nkb);
           }
         }
         if (!ok) break;
@@ -323,7 +335,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     // -------------------------------------------------------------- softmax
     const int map = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t ts = tmem + map * 128 + lanes, to = tmem + TM_O + map * W + lanes;
+    const uint32_t to = tmem + TM_O + map * W + lanes;
     const float scale = 1.4426950408889634f * rsqrtf((float)D);
     const unsigned long long scale2 = f2_pack(scale, scale);
     float* sums = reinterpret_cast<float*>(smem + L::OFF_L);
@@ -334,26 +346,31 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const int nkb = (t.y + BKEY - 1) / BKEY;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nkb; j++, ib++) {
-        ok = __all_sync(0xffffffffu, mbar_wait(s_full(map), ib & 1, abort_flag, status, 74));
+        const uint32_t ts = tmem + map * 128 + (ib & 1) * BKEY + lanes;
+        ok = __all_sync(0xffffffffu, mbar_wait(s_full(map, ib), (ib >> 1) & 1, abort_flag, status, 74));
         if (!ok) break;
         tc_fence_after();
-        uint32_t r[128];
-#pragma unroll
-        for (int c = 0; c < 4; c++) ld32(ts + 32 * c, r + 32 * c);
+        uint32_t r[BKEY];
+        ld32(ts, r);
+        ld32(ts + 32, r + 32);
         wait_ld();
         const int left = t.y - j * BKEY;  // keys of this block and behind
         if (left < BKEY) {
 #pragma unroll
-          for (int e = 0; e < 128; e++) r[e] = e < left ? r[e] : 0xff800000u;
+          for (int e = 0; e < BKEY; e++) r[e] = e < left ? r[e] : 0xff800000u;
         }
         float m0 = m, m1 = -INFINITY;
-        chunk_max<128>(m0, m1, r, 128);
+        chunk_max<BKEY>(m0, m1, r, BKEY);
         m0 = fmaxf(m0, m1);
         if (j == 0) {
           m = m0;
         } else if (__any_sync(0xffffffffu, (m0 - m) * scale > GROW)) {
           const float f = ex2((m - m0) * scale);
           const unsigned long long f2 = f2_pack(f, f);
+          // The result of the blocks before, complete.
+          ok = __all_sync(0xffffffffu, mbar_wait(o_done(map), (ib - 1) & 1, abort_flag, status, 79));
+          if (!ok) break;
+          tc_fence_after();
           m = m0;
           l *= f;
 #pragma unroll 1
@@ -374,7 +391,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         const unsigned long long off = f2_pack(-m * scale, -m * scale);
         unsigned long long s0 = 0, s1 = 0;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
+        for (int c = 0; c < BKEY / 32; c++) {
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 16; e++) {
@@ -396,18 +413,18 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         l += a + b;
         if (map == 0 && left < BKEY && left % 16 != 0) {
           // The values between the last key and the end of its 16.
-          ok = __all_sync(0xffffffffu, mbar_wait(v_full(ib & 1), (ib >> 1) & 1, abort_flag, status, 75));
+          ok = __all_sync(0xffffffffu, mbar_wait(v_full(ib % KV), (ib / KV) & 1, abort_flag, status, 75));
           if (!ok) break;
           const int rows = 16 - left % 16;
-          uint8_t* v = smem + L::OFF_V + (ib & 1) * OP + left * 128;
+          uint8_t* v = smem + L::OFF_V + (ib % KV) * L::KB + left * 128;
           for (int e = row; e < rows * 8 * NT; e += 128)
-            *reinterpret_cast<uint4*>(v + e / (rows * 8) * TILE + e % (rows * 8) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(v + e / (rows * 8) * KTILE + e % (rows * 8) * 16) = make_uint4(0, 0, 0, 0);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(map));
+        if (lane == 0) mbar_arrive(p_full(map, ib));
       }
       if (!ok) break;
       // ------------------------------------------------------------ result
@@ -499,10 +516,10 @@ template <class T, int D>
 static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
   auto enc = encode_fn();
   if (!enc) return cudaErrorNotSupported;
-  auto encode = [&](CUtensorMap* map, const void* ptr, int heads, long ld) {
+  auto encode = [&](CUtensorMap* map, const void* ptr, int heads, long ld, int rows) {
     const cuuint64_t dims[2] = {(cuuint64_t)heads * 2 * D, (cuuint64_t)p.T};
     const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {64, 128};
+    const cuuint32_t box[2] = {64, (cuuint32_t)rows};
     const cuuint32_t estr[2] = {1, 1};
     const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -512,7 +529,7 @@ static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
   };
   CUtensorMap mq, mk, mv;
   const int kvh = p.heads / p.group;
-  if (!encode(&mq, p.q, p.heads, p.q_stride) || !encode(&mk, p.k, kvh, p.k_stride) || !encode(&mv, p.v, kvh, p.v_stride))
+  if (!encode(&mq, p.q, p.heads, p.q_stride, BQ) || !encode(&mk, p.k, kvh, p.k_stride, BKEY) || !encode(&mv, p.v, kvh, p.v_stride, BKEY))
     return cudaErrorInvalidValue;
   static std::mutex mu;
   static int sms[64] = {};
