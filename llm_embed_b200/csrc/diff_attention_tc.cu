@@ -16,7 +16,9 @@
 // head, 16 a clock and SM.
 //
 //   warp 0      producer: TMA loads of Q (two stages), K and V (four each)
-//   warp 1      TMEM allocation; MMAs: S_i = Q_i K_i^T, O_i += P_i V
+//   warps 1, 2  MMAs of a map each: S_i = Q_i K_i^T, O_i += P_i V (one warp
+//               for both spent more time on its waits than the tensor cores
+//               on their work: 2070 clocks a block, 775 of them busy)
 //   warp 3      finds the tiles' sequences and publishes them in a ring
 //   warps 4-7   map 1, warps 8-11 map 2: softmax; then each group combines
 //               half of the columns of O_1 and O_2, norms and stores them
@@ -64,10 +66,10 @@ struct Lay {
   static constexpr int OFF_RING = OFF_L + 2 * 2 * 2 * 128 * 4;
   static constexpr int OFF_BAR = OFF_RING + RING * 16;
   // q_full q_empty [2 each], k_full k_empty v_full v_empty [KV each], s_full
-  // p_full [2 maps][2], o_done [2], o_full o_empty sum_full sq_full, ring_full
+  // p_full [2 maps][2], o_done [2], o_full o_empty sum_full sq_full v_fixed, ring_full
   // ring_empty [RING]
   static constexpr int B_Q = 0, B_K = 4, B_V = B_K + 2 * KV, B_S = B_V + 2 * KV, B_P = B_S + 4, B_D = B_P + 4,
-                       B_O = B_D + 2, B_R = B_O + 4, NBAR = B_R + 2 * RING;
+                       B_O = B_D + 2, B_R = B_O + 5, NBAR = B_R + 2 * RING;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;
   static_assert(ALLOC <= 232448, "shared memory of one CTA");
@@ -139,7 +141,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   auto s_full = [&](int i, uint32_t b) { return bar0 + 8 * (L::B_S + 2 * i + (b & 1)); };
   auto p_full = [&](int i, uint32_t b) { return bar0 + 8 * (L::B_P + 2 * i + (b & 1)); };
   auto o_done = [&](int i) { return bar0 + 8 * (L::B_D + i); };
-  const uint32_t o_full = bar0 + 8 * L::B_O, o_empty = o_full + 8, sum_full = o_full + 16, sq_full = o_full + 24;
+  const uint32_t o_full = bar0 + 8 * L::B_O, o_empty = o_full + 8, sum_full = o_full + 16, sq_full = o_full + 24,
+                 v_fixed = o_full + 32;
   auto ring_full = [&](int e) { return bar0 + 8 * (L::B_R + e); };
   auto ring_empty = [&](int e) { return bar0 + 8 * (L::B_R + RING + e); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC);
@@ -150,13 +153,29 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int i = 0; i <= L::B_O; i++) mbar_init(bar0 + 8 * i, i >= L::B_P && i < L::B_D ? 4 : 1);  // p_full: four warps
+    for (int i = 0; i < 2; i++) {
+      mbar_init(q_full(i), 1);
+      mbar_init(q_empty(i), 2);  // the two maps' MMAs
+      mbar_init(o_done(i), 1);
+      for (int b = 0; b < 2; b++) {
+        mbar_init(s_full(i, b), 1);
+        mbar_init(p_full(i, b), 4);
+      }
+    }
+    for (int s = 0; s < KV; s++) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 2);
+      mbar_init(v_full(s), 1);
+      mbar_init(v_empty(s), 2);
+    }
+    mbar_init(o_full, 2);
+    mbar_init(v_fixed, 4);
     mbar_init(o_empty, 8);
     mbar_init(sum_full, 8);
     mbar_init(sq_full, 8);
     for (int e = 0; e < RING; e++) {
       mbar_init(ring_full(e), 1);
-      mbar_init(ring_empty(e), 10);  // producer, MMA, eight softmax warps
+      mbar_init(ring_empty(e), 11);  // producer, two MMA, eight softmax warps
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -240,54 +259,40 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
         n++;
       }
-    } else if (warp == 1) {
+    } else {
       // ---------------------------------------------------------------- MMA
+      const int i = warp - 1;  // map
       const bool issuer = elect_one();
-      uint32_t n = 0, ib = 0;
+      const uint32_t s_tm = tmem + i * 128, o_tm = tmem + TM_O + i * W;
+      uint32_t n = 0, ib = 0, fixed = 0;
       int4 t;
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity, int site) {
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, site));
+        ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, site));
         return ok;
       };
+      // Operand descriptors (their addresses count 16-byte units).  Map i of an
+      // operand with d = 64 is a tile of its own, with d = 32 half of the
+      // 128-byte rows.  V [keys][64] tiles side by side: KTILE bytes from one
+      // 64-column group to the next (leading offset), 16 keys = 2048 bytes.
+      const uint64_t q0 = sw128_desc(sbase + L::OFF_Q + i * (D == 64 ? QTILE : 64));
+      const uint64_t k0 = sw128_desc(sbase + L::OFF_K + i * (D == 64 ? KTILE : 64));
+      const uint64_t v0 = (sw128_desc(sbase + L::OFF_V) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(KTILE >> 4) << 16);
       while (ok && next_tile(n, t)) {
-        const int qs = n & 1, nkb = (t.y + BKEY - 1) / BKEY;
-        // Map i of an operand with d = 64 is a tile of its own, with d = 32
-        // half of the 128-byte rows.
-        auto issue_s = [&](int i, uint32_t b) {  // S_i of block number b
+        const uint32_t qs = n & 1;
+        const int nkb = (t.y + BKEY - 1) / BKEY;
+        const uint64_t qd = q0 + qs * (L::QB / 16);
+        // S of block number b, once its keys are there; then they are free,
+        // with the tile's last block the queries too.
+        auto scores = [&](uint32_t b, bool last) {
+          if (!wait(k_full(b % KV), (b / KV) & 1, 66)) return;
+          tc_fence_after();
           if (issuer) {
-            const uint64_t qd = sw128_desc(sbase + L::OFF_Q + qs * L::QB + i * (D == 64 ? QTILE : 64));
-            const uint64_t kd = sw128_desc(sbase + L::OFF_K + (b % KV) * L::KB + i * (D == 64 ? KTILE : 64));
+            const uint64_t kd = k0 + (b % KV) * (L::KB / 16);
 #pragma unroll
             for (int kk = 0; kk < D / 16; kk++)
-              mma_f16(tmem + i * 128 + (b & 1) * BKEY, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk != 0);
+              mma_f16(s_tm + (b & 1) * BKEY, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk != 0);
             mma_commit(s_full(i, b));
-          }
-          __syncwarp();
-        };
-        auto issue_pv = [&](int i, uint32_t b, int steps, bool first) {
-          if (issuer) {
-            // V [keys][64] tiles side by side: KTILE bytes from one 64-column
-            // group to the next (leading offset), 16 keys = 2048 bytes.
-            const uint64_t vd = (sw128_desc(sbase + L::OFF_V + (b % KV) * L::KB) & ~((uint64_t)0x3FFF << 16)) |
-                                ((uint64_t)(KTILE >> 4) << 16);
-#pragma unroll
-            for (int kk = 0; kk < BKEY / 16; kk++)
-              if (kk < steps)
-                mma_ts(tmem + TM_O + i * W, tmem + i * 128 + (b & 1) * BKEY + kk * 8, vd + kk * (2048 >> 4), IDESC_O,
-                       !(first && kk == 0));
-            mma_commit(o_done(i));
-          }
-          __syncwarp();
-        };
-        auto k_ready = [&](uint32_t b) {
-          if (!wait(k_full(b % KV), (b / KV) & 1, 66)) return false;
-          tc_fence_after();
-          return true;
-        };
-        // K of block b is read; Q too with the tile's last.
-        auto k_done = [&](uint32_t b, bool last) {
-          if (issuer) {
             mma_commit(k_empty(b % KV));
             if (last) mma_commit(q_empty(qs));
           }
@@ -295,38 +300,36 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         };
         if (!wait(q_full(qs), (n >> 1) & 1, 65)) break;
         // The scores run two blocks ahead of the values.
-        for (int j = 0; j < 2 && j < nkb && ok; j++)
-          if (k_ready(ib + j)) {
-            issue_s(0, ib + j);
-            issue_s(1, ib + j);
-            k_done(ib + j, j + 1 == nkb);
-          }
-        if (!ok) break;
+        scores(ib, nkb == 1);
+        if (ok && nkb > 1) scores(ib + 1, nkb == 2);
+        if (!ok || !wait(o_empty, (n & 1) ^ 1, 68)) break;
         for (int j = 0; j < nkb; j++, ib++) {
-          const int steps = min(BKEY, t.y - j * BKEY + 15) / 16;
-          const bool more = j + 2 < nkb;
-          if (!wait(v_full(ib % KV), (ib / KV) & 1, 67) || (j == 0 && !wait(o_empty, (n & 1) ^ 1, 68)) ||
-              !wait(p_full(0, ib), (ib >> 1) & 1, 69))
-            break;
+          const int left = t.y - j * BKEY, steps = min(BKEY, left + 15) / 16;
+          if (!wait(v_full(ib % KV), (ib / KV) & 1, 67)) break;
+          if (left < BKEY && left % 16 != 0 && !wait(v_fixed, fixed++ & 1, 69)) break;
+          if (!wait(p_full(i, ib), (ib >> 1) & 1, 73)) break;
           tc_fence_after();
-          issue_pv(0, ib, steps, j == 0);
-          if (more) {
-            if (!k_ready(ib + 2)) break;
-            issue_s(0, ib + 2);
+          if (issuer) {
+            const uint64_t vd = v0 + (ib % KV) * (L::KB / 16);
+            const uint32_t pt = s_tm + (ib & 1) * BKEY;
+            if (steps == BKEY / 16) {
+#pragma unroll
+              for (int kk = 0; kk < BKEY / 16; kk++)
+                mma_ts(o_tm, pt + kk * 8, vd + kk * (2048 / 16), IDESC_O, j != 0 || kk != 0);
+            } else {
+              for (int kk = 0; kk < steps; kk++)
+                mma_ts(o_tm, pt + kk * 8, vd + kk * (2048 / 16), IDESC_O, j != 0 || kk != 0);
+            }
+            mma_commit(o_done(i));
+            mma_commit(v_empty(ib % KV));
+            if (j + 1 == nkb) mma_commit(o_full);
           }
-          if (!wait(p_full(1, ib), (ib >> 1) & 1, 73)) break;
-          tc_fence_after();
-          issue_pv(1, ib, steps, j == 0);
-          if (issuer) mma_commit(v_empty(ib % KV));
           __syncwarp();
-          if (more) {
-            issue_s(1, ib + 2);
-            k_done(ib + 2, j + 3 == nkb);
+          if (j + 2 < nkb) {
+            scores(ib + 2, j + 3 == nkb);
+            if (!ok) break;
           }
         }
-        if (!ok) break;
-        if (issuer) mma_commit(o_full);
-        __syncwarp();
         n++;
       }
     }
@@ -420,6 +423,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           for (int e = row; e < rows * 8 * NT; e += 128)
             *reinterpret_cast<uint4*>(v + e / (rows * 8) * KTILE + e % (rows * 8) * 16) = make_uint4(0, 0, 0, 0);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_fixed);
         }
         wait_st();
         tc_fence_before();
