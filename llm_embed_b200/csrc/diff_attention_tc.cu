@@ -3,7 +3,8 @@
 //   A_i = softmax(q_i k_i^T / sqrt(d)), o = (A_1 - lambda A_2) v, then the
 //   head's norm (diff_attention.cu has the formulas in full).
 //
-// Persistent kernel, one CTA per SM.  A tile is 128 queries of one head and
+// One CTA per SM, which goes from tile to tile (cluster launch control hands
+// out the grid's CTAs that have not started).  A tile is 128 queries of one head and
 // sequence; its two maps are two chains that share the keys' and values'
 // loads and take turns on the tensor cores: while one map's scores are
 // exponentiated, the other's products run.  A thread of a map's warpgroup has
@@ -19,7 +20,7 @@
 //   warps 1, 2  MMAs of a map each: S_i = Q_i K_i^T, O_i += P_i V (one warp
 //               for both spent more time on its waits than the tensor cores
 //               on their work: 2070 clocks a block, 775 of them busy)
-//   warp 3      finds the tiles' sequences and publishes them in a ring
+//   warp 3      takes the tiles, finds their sequences and publishes them
 //   warps 4-7   map 1, warps 8-11 map 2: softmax; then each group combines
 //               half of the columns of O_1 and O_2, norms and stores them
 // TMEM (512 columns): two buffers of S_i / P_i for each map (64 each), O_1,
@@ -51,7 +52,7 @@ constexpr int BQ = 128, BKEY = 64;
 constexpr int QTILE = 128 * 128, KTILE = 64 * 128;  // bytes of 128 and 64 rows x 64 columns
 constexpr int KV = 4;                               // stages of K and of V
 constexpr int NTHREADS = 384;
-constexpr int RING = 3;
+constexpr int RING = 1;
 constexpr float GROW = 8.f;  // log2 of the growth that moves the maximum
 
 template <int D>
@@ -64,12 +65,13 @@ struct Lay {
   static constexpr int OFF_V = OFF_K + KV * KB;  // [KV]
   static constexpr int OFF_L = OFF_V + KV * KB;  // sums [2 tiles][2 maps][128], squares likewise
   static constexpr int OFF_RING = OFF_L + 2 * 2 * 2 * 128 * 4;
-  static constexpr int OFF_BAR = OFF_RING + RING * 16;
+  static constexpr int OFF_NORM = OFF_RING + RING * 16 + 16;  // the next item's answer; norm weights [2d]
+  static constexpr int OFF_BAR = OFF_NORM + 2 * D * 4;
   // q_full q_empty [2 each], k_full k_empty v_full v_empty [KV each], s_full
   // p_full [2 maps][2], o_done [2], o_full o_empty sum_full sq_full v_fixed, ring_full
-  // ring_empty [RING]
+  // ring_empty [RING], turn [2 maps][4 quarters], next item
   static constexpr int B_Q = 0, B_K = 4, B_V = B_K + 2 * KV, B_S = B_V + 2 * KV, B_P = B_S + 4, B_D = B_P + 4,
-                       B_O = B_D + 2, B_R = B_O + 5, NBAR = B_R + 2 * RING;
+                       B_O = B_D + 2, B_R = B_O + 5, B_T = B_R + 2 * RING, NBAR = B_T + 9;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;
   static_assert(ALLOC <= 232448, "shared memory of one CTA");
@@ -122,7 +124,7 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* w, bool wide) {
 template <class T, int D>
 __global__ void __launch_bounds__(NTHREADS, 1)
     diff_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                   const __grid_constant__ CUtensorMap tmap_v, DiffParams p, int tiles, int wide) {
+                   const __grid_constant__ CUtensorMap tmap_v, DiffParams p, int wide) {
   using L = Lay<D>;
   constexpr int NT = L::NT, W = 2 * D;
   constexpr uint32_t FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0;
@@ -145,6 +147,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                  v_fixed = o_full + 32;
   auto ring_full = [&](int e) { return bar0 + 8 * (L::B_R + e); };
   auto ring_empty = [&](int e) { return bar0 + 8 * (L::B_R + RING + e); };
+  auto turn = [&](int i, int q) { return bar0 + 8 * (L::B_T + 4 * i + q); };
+  const uint32_t item_bar = turn(0, 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC + 4);
   int4* ring = reinterpret_cast<int4*>(smem + L::OFF_RING);  // {t0, len, q0, head}, len 0: no more
@@ -170,6 +174,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
     mbar_init(o_full, 2);
     mbar_init(v_fixed, 4);
+    for (int i = 0; i < 9; i++) mbar_init(turn(0, i), 1);  // and item_bar
     mbar_init(o_empty, 8);
     mbar_init(sum_full, 8);
     mbar_init(sq_full, 8);
@@ -189,7 +194,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
-  pdl_trigger();
+  // No pdl_trigger: the next kernel waits for this one's CTAs, started or
+  // cancelled, to be done.
+  if (threadIdx.x < W && p.norm_w) reinterpret_cast<float*>(smem + L::OFF_NORM)[threadIdx.x] = p.norm_w[threadIdx.x];
+  __syncthreads();
 
   // The next tile of the ring, for a whole warp; false at the end.
   auto next_tile = [&](uint32_t n, int4& tile) -> bool {
@@ -220,15 +228,46 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         n++;
         return true;
       };
+      auto ring_free = [&]() -> bool {  // every reader has taken the last tile
+        return __all_sync(0xffffffffu,
+                          mbar_wait(ring_empty(n % RING), ((n / RING) & 1) ^ 1, abort_flag, status, 82)) != 0;
+      };
+      // The first item is the CTA's own; further ones are CTAs of the grid that
+      // have not started, cancelled one at a time, so that the items go to
+      // whichever SM is free.
+      const uint32_t answer = sbase + L::OFF_RING + RING * 16;
       Where w{};
       int last = -1;
       bool found = false, ok = true;
-      const long items = (long)tiles * p.heads;
-      for (long item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        const int tile = (int)(item / p.heads), head = (int)(item - (long)tile * p.heads);
+      uint32_t item = blockIdx.x;
+      for (uint32_t k = 0;; k++) {
+        const int tile = (int)(item / (uint32_t)p.heads), head = (int)(item - (uint32_t)tile * p.heads);
         if (tile != last) found = find_block(p, tile, BQ, w) && w.len >= p.min_len;
         last = tile;
-        if (found) ok = publish(make_int4(w.t0, w.len, w.q0, head));
+        if (found) ok = publish(make_int4(w.t0, w.len, w.q0, head)) && ring_free();
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(item_bar, 16);
+          asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::
+                           "r"(answer),
+                       "r"(item_bar)
+                       : "memory");
+        }
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, mbar_wait(item_bar, k & 1, abort_flag, status, 81));
+        if (!ok) break;
+        uint64_t lo, hi;
+        uint32_t more;
+        asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(answer) : "memory");
+        asm volatile(
+            "{\n.reg .b128 a;\n.reg .pred p;\nmov.b128 a, {%2, %3};\n"
+            "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\nselp.u32 %0, 1, 0, p;\n"
+            "mov.u32 %1, 0;\n"
+            "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n}\n"
+            : "=r"(more), "=&r"(item)
+            : "l"(lo), "l"(hi));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read before the next answer
+        if (!more) break;
       }
       if (ok) publish(make_int4(0, 0, 0, 0));
     } else if (warp == 0) {
@@ -348,6 +387,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     while (ok && next_tile(n, t)) {
       const int nkb = (t.y + BKEY - 1) / BKEY;
       float m = -INFINITY, l = 0.f;
+      const float lambda = p.lambda[t.w];
       for (int j = 0; j < nkb; j++, ib++) {
         const uint32_t ts = tmem + map * 128 + (ib & 1) * BKEY + lanes;
         ok = __all_sync(0xffffffffu, mbar_wait(s_full(map, ib), (ib >> 1) & 1, abort_flag, status, 74));
@@ -362,9 +402,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
           for (int e = 0; e < BKEY; e++) r[e] = e < left ? r[e] : 0xff800000u;
         }
-        float m0 = m, m1 = -INFINITY;
-        chunk_max<BKEY>(m0, m1, r, BKEY);
-        m0 = fmaxf(m0, m1);
+        float m0 = m, m1 = __uint_as_float(r[0]), m2 = __uint_as_float(r[1]), m3 = __uint_as_float(r[2]);
+#pragma unroll
+        for (int e = 0; e < BKEY; e += 8) {
+          m0 = max3(m0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+          m1 = max3(m1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+          m2 = max3(m2, __uint_as_float(r[e + 4]), __uint_as_float(r[e + 5]));
+          m3 = max3(m3, __uint_as_float(r[e + 6]), __uint_as_float(r[e + 7]));
+        }
+        m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
         if (j == 0) {
           m = m0;
         } else if (__any_sync(0xffffffffu, (m0 - m) * scale > GROW)) {
@@ -392,24 +438,39 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           }
         }
         const unsigned long long off = f2_pack(-m * scale, -m * scale);
+#pragma unroll
+        for (int e = 0; e < BKEY; e += 2) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), scale2, off), x0, x1);
+          r[e] = __float_as_uint(x0);
+          r[e + 1] = __float_as_uint(x1);
+        }
+        // The maps take turns at the exponentials, so that one's other work
+        // runs beside them; the turn is passed on a little before the end.
+        ok = __all_sync(0xffffffffu, mbar_wait(turn(map, quarter), (ib & 1) ^ (map ^ 1), abort_flag, status, 80));
+        if (!ok) break;
+#pragma unroll
+        for (int e = 0; e < BKEY; e++) {
+          if (e == BKEY - 12) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(turn(map ^ 1, quarter));
+          }
+          r[e] = __float_as_uint(ex2(__uint_as_float(r[e])));
+        }
         unsigned long long s0 = 0, s1 = 0;
 #pragma unroll
-        for (int c = 0; c < BKEY / 32; c++) {
+        for (int c = 0; c < BKEY; c += 32) {
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 16; e++) {
-            float x0, x1;
-            const int at = 32 * c + 2 * e;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(r[at]), __uint_as_float(r[at + 1])), scale2, off), x0, x1);
-            x0 = ex2(x0);
-            x1 = ex2(x1);
+            const float x0 = __uint_as_float(r[c + 2 * e]), x1 = __uint_as_float(r[c + 2 * e + 1]);
+            w[e] = pack2<T>(x0, x1);
             if (e & 1)
               s1 = f2_add(s1, f2_pack(x0, x1));
             else
               s0 = f2_add(s0, f2_pack(x0, x1));
-            w[e] = pack2<T>(x0, x1);
           }
-          st16(ts + 16 * c, w);
+          st16(ts + c / 2, w);
         }
         float a, b;
         f2_unpack(f2_add(s0, s1), a, b);
@@ -448,7 +509,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       ok = meet(sum_full, 77) && __all_sync(0xffffffffu, mbar_wait(o_full, n & 1, abort_flag, status, 76));
       if (!ok) break;
       tc_fence_after();
-      const float w1 = 1.f / sum[row], w2 = p.lambda[t.w] / sum[128 + row];
+      const float w1 = 1.f / sum[row], w2 = lambda / sum[128 + row];
       const uint32_t o1 = tmem + TM_O + lanes + map * D, o2 = o1 + W;
       float o[D], ss = 0.f;
 #pragma unroll
@@ -466,18 +527,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty);
-      const float* nw = p.norm_w;
-      if (nw) {
+      if (p.norm_w) {
+        const float4* nw = reinterpret_cast<const float4*>(smem + L::OFF_NORM) + map * (D / 4);
         sq[map * 128 + row] = ss;
         ok = meet(sq_full, 78);
         if (!ok) break;
-        const float f = p.out_scale * rsqrtf((sq[row] + sq[128 + row]) / (float)W + p.eps);
+        const float f = p.out_scale * rsqrtf((sq[row] + sq[128 + row]) * (1.f / W) + p.eps);
 #pragma unroll
-        for (int c = 0; c < D; c += 8) {
-          float w[8];
-          load_f32x8(nw + map * D + c, w);
-#pragma unroll
-          for (int e = 0; e < 8; e++) o[c + e] *= f * w[e];
+        for (int c = 0; c < D; c += 4) {
+          const float4 w = nw[c / 4];
+          o[c] *= f * w.x, o[c + 1] *= f * w.y, o[c + 2] *= f * w.z, o[c + 3] *= f * w.w;
         }
       }
       if (t.z + row < t.y) {
@@ -537,26 +596,26 @@ static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
   if (!encode(&mq, p.q, p.heads, p.q_stride, BQ) || !encode(&mk, p.k, kvh, p.k_stride, BKEY) || !encode(&mv, p.v, kvh, p.v_stride, BKEY))
     return cudaErrorInvalidValue;
   static std::mutex mu;
-  static int sms[64] = {};
+  static uint64_t attr_set = 0;  // per-device bit: the attribute is a per-device setting
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 64) return cudaErrorInvalidDevice;
   {
     std::lock_guard<std::mutex> lk(mu);
-    if (sms[dev] == 0) {
-      cudaError_t e =
+    if (dev >= 64 || !(attr_set >> dev & 1)) {
+      const cudaError_t e =
           cudaFuncSetAttribute(diff_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::ALLOC);
-      if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
       if (e != cudaSuccess) return e;
+      if (dev < 64) attr_set |= 1ull << dev;
     }
   }
   const int tiles = block_count(p.T, p.nseq, BQ);
   const long items = (long)tiles * p.heads;
+  if (items > 0x7fffffff) return cudaErrorInvalidValue;
   const int wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.o_stride % 16 == 0;
   cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)(items < sms[dev] ? items : sms[dev])), dim3(NTHREADS),
+  const cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)items), dim3(NTHREADS),
                                             Lay<D>::ALLOC, s, attr);
-  return cudaLaunchKernelEx(&cfg, diff_tc_kernel<T, D>, mq, mk, mv, p, tiles, wide);
+  return cudaLaunchKernelEx(&cfg, diff_tc_kernel<T, D>, mq, mk, mv, p, wide);
 }
 
 }  // namespace dtc
