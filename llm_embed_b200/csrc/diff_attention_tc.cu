@@ -21,8 +21,9 @@
 //               for both spent more time on its waits than the tensor cores
 //               on their work: 2070 clocks a block, 775 of them busy)
 //   warp 3      takes the tiles, finds their sequences and publishes them
-//   warps 4-7   map 1, warps 8-11 map 2: softmax; then each group combines
-//               half of the columns of O_1 and O_2, norms and stores them
+//   warps 4-7   softmax of map 1, warps 8-11 of map 2
+//   warps 12-15 combine O_1 and O_2, norm and store, beside the next tile's
+//               first two blocks
 // TMEM (512 columns): two buffers of S_i / P_i for each map (64 each), O_1,
 // O_2 (2d each).  A map's MMAs run in the order they are issued - S of block
 // j + 2 after P.V of block j, whose buffer it takes - so a map has a block of
@@ -51,7 +52,7 @@ using namespace dif;
 constexpr int BQ = 128, BKEY = 64;
 constexpr int QTILE = 128 * 128, KTILE = 64 * 128;  // bytes of 128 and 64 rows x 64 columns
 constexpr int KV = 4;                               // stages of K and of V
-constexpr int NTHREADS = 384;
+constexpr int NTHREADS = 512;
 constexpr int RING = 1;
 constexpr float GROW = 8.f;  // log2 of the growth that moves the maximum
 
@@ -63,15 +64,15 @@ struct Lay {
   static constexpr int OFF_Q = 0;         // [2]
   static constexpr int OFF_K = 2 * QB;    // [KV]
   static constexpr int OFF_V = OFF_K + KV * KB;  // [KV]
-  static constexpr int OFF_L = OFF_V + KV * KB;  // sums [2 tiles][2 maps][128], squares likewise
-  static constexpr int OFF_RING = OFF_L + 2 * 2 * 2 * 128 * 4;
+  static constexpr int OFF_L = OFF_V + KV * KB;  // sums [2 tiles][2 maps][128]
+  static constexpr int OFF_RING = OFF_L + 2 * 2 * 128 * 4;
   static constexpr int OFF_NORM = OFF_RING + RING * 16 + 16;  // the next item's answer; norm weights [2d]
   static constexpr int OFF_BAR = OFF_NORM + 2 * D * 4;
   // q_full q_empty [2 each], k_full k_empty v_full v_empty [KV each], s_full
-  // p_full [2 maps][2], o_done [2], o_full o_empty sum_full sq_full v_fixed, ring_full
+  // p_full [2 maps][2], o_done [2], o_full o_empty sum_full v_fixed, ring_full
   // ring_empty [RING], turn [2 maps][4 quarters], next item
   static constexpr int B_Q = 0, B_K = 4, B_V = B_K + 2 * KV, B_S = B_V + 2 * KV, B_P = B_S + 4, B_D = B_P + 4,
-                       B_O = B_D + 2, B_R = B_O + 5, B_T = B_R + 2 * RING, NBAR = B_T + 9;
+                       B_O = B_D + 2, B_R = B_O + 4, B_T = B_R + 2 * RING, NBAR = B_T + 9;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;
   static_assert(ALLOC <= 232448, "shared memory of one CTA");
@@ -143,8 +144,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   auto s_full = [&](int i, uint32_t b) { return bar0 + 8 * (L::B_S + 2 * i + (b & 1)); };
   auto p_full = [&](int i, uint32_t b) { return bar0 + 8 * (L::B_P + 2 * i + (b & 1)); };
   auto o_done = [&](int i) { return bar0 + 8 * (L::B_D + i); };
-  const uint32_t o_full = bar0 + 8 * L::B_O, o_empty = o_full + 8, sum_full = o_full + 16, sq_full = o_full + 24,
-                 v_fixed = o_full + 32;
+  const uint32_t o_full = bar0 + 8 * L::B_O, o_empty = o_full + 8, sum_full = o_full + 16, v_fixed = o_full + 24;
   auto ring_full = [&](int e) { return bar0 + 8 * (L::B_R + e); };
   auto ring_empty = [&](int e) { return bar0 + 8 * (L::B_R + RING + e); };
   auto turn = [&](int i, int q) { return bar0 + 8 * (L::B_T + 4 * i + q); };
@@ -175,12 +175,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     mbar_init(o_full, 2);
     mbar_init(v_fixed, 4);
     for (int i = 0; i < 9; i++) mbar_init(turn(0, i), 1);  // and item_bar
-    mbar_init(o_empty, 8);
+    mbar_init(o_empty, 4);
     mbar_init(sum_full, 8);
-    mbar_init(sq_full, 8);
     for (int e = 0; e < RING; e++) {
       mbar_init(ring_full(e), 1);
-      mbar_init(ring_empty(e), 11);  // producer, two MMA, eight softmax warps
+      mbar_init(ring_empty(e), 15);  // producer, two MMA, eight softmax, four epilogue warps
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -209,10 +208,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     return tile.y > 0;
   };
 
-  // 384 threads of 168 registers at launch: the softmax threads hold 128
-  // scores each.
+  // 512 threads of 128 registers at launch; the softmax threads take what the
+  // others leave: 56 + 2 * 176 + 104 = 4 * 128.
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 3) {
       // -------------------------------------------------------------- tiles
       if (blockIdx.x == 0) check_offsets(p, 32);
@@ -372,8 +371,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         n++;
       }
     }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     // -------------------------------------------------------------- softmax
     const int map = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -387,7 +386,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     while (ok && next_tile(n, t)) {
       const int nkb = (t.y + BKEY - 1) / BKEY;
       float m = -INFINITY, l = 0.f;
-      const float lambda = p.lambda[t.w];
       for (int j = 0; j < nkb; j++, ib++) {
         const uint32_t ts = tmem + map * 128 + (ib & 1) * BKEY + lanes;
         ok = __all_sync(0xffffffffu, mbar_wait(s_full(map, ib), (ib >> 1) & 1, abort_flag, status, 74));
@@ -493,60 +491,77 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (lane == 0) mbar_arrive(p_full(map, ib));
       }
       if (!ok) break;
-      // ------------------------------------------------------------ result
-      // The groups exchange their rows' sums (two buffers: a group may be at
-      // the next tile's before the other has read these) and take half of the
-      // columns each.
-      float* sum = sums + (n & 1) * 256;
-      float* sq = sums + 512 + (n & 1) * 256;
-      // Eight warps meet at a barrier whose wait is bounded as all others.
-      auto meet = [&](uint32_t bar, int site) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
-        return __all_sync(0xffffffffu, mbar_wait(bar, n & 1, abort_flag, status, site)) != 0;
-      };
-      sum[map * 128 + row] = l;
-      ok = meet(sum_full, 77) && __all_sync(0xffffffffu, mbar_wait(o_full, n & 1, abort_flag, status, 76));
-      if (!ok) break;
+      // The row's sum, for the epilogue (two buffers: it has read a tile's
+      // before the next one's results can be complete).
+      sums[(n & 1) * 256 + map * 128 + row] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sum_full);
+      n++;
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    // ------------------------------------------------------------- epilogue
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t o1 = tmem + TM_O + ((uint32_t)(quarter * 32) << 16);
+    const float* sums = reinterpret_cast<const float*>(smem + L::OFF_L);
+    const float4* nw = reinterpret_cast<const float4*>(smem + L::OFF_NORM);
+    uint32_t n = 0;
+    int4 t;
+    while (next_tile(n, t)) {
+      const float lambda = p.lambda[t.w];
+      if (!__all_sync(0xffffffffu, mbar_wait(sum_full, n & 1, abort_flag, status, 77)) ||
+          !__all_sync(0xffffffffu, mbar_wait(o_full, n & 1, abort_flag, status, 76)))
+        break;
       tc_fence_after();
-      const float w1 = 1.f / sum[row], w2 = lambda / sum[128 + row];
-      const uint32_t o1 = tmem + TM_O + lanes + map * D, o2 = o1 + W;
-      float o[D], ss = 0.f;
-#pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      const float* sum = sums + (n & 1) * 256;
+      const float w1 = 1.f / sum[row], w2 = -lambda / sum[128 + row];
+      // o of 32 columns; a second look at them costs less than the registers
+      // that would keep them.
+      auto combine = [&](int c, float (&o)[32]) {
         uint32_t a[32], b[32];
         ld32(o1 + c, a);
-        ld32(o2 + c, b);
+        ld32(o1 + W + c, b);
         wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-          o[c + e] = fmaf(__uint_as_float(a[e]), w1, -__uint_as_float(b[e]) * w2);
-          ss = fmaf(o[c + e], o[c + e], ss);
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(o_empty);
+        for (int e = 0; e < 32; e++) o[e] = fmaf(__uint_as_float(a[e]), w1, __uint_as_float(b[e]) * w2);
+      };
+      float f = 1.f;
       if (p.norm_w) {
-        const float4* nw = reinterpret_cast<const float4*>(smem + L::OFF_NORM) + map * (D / 4);
-        sq[map * 128 + row] = ss;
-        ok = meet(sq_full, 78);
-        if (!ok) break;
-        const float f = p.out_scale * rsqrtf((sq[row] + sq[128 + row]) * (1.f / W) + p.eps);
+        float ss = 0.f;
 #pragma unroll
-        for (int c = 0; c < D; c += 4) {
-          const float4 w = nw[c / 4];
-          o[c] *= f * w.x, o[c + 1] *= f * w.y, o[c + 2] *= f * w.z, o[c + 3] *= f * w.w;
+        for (int c = 0; c < W; c += 32) {
+          float o[32];
+          combine(c, o);
+#pragma unroll
+          for (int e = 0; e < 32; e++) ss = fmaf(o[e], o[e], ss);
         }
+        f = p.out_scale * rsqrtf(ss * (1.f / W) + p.eps);
       }
-      if (t.z + row < t.y) {
-        T* out = static_cast<T*>(p.out) + (long)(t.x + t.z + row) * p.o_stride + (long)t.w * W + map * D;
+      T* out = static_cast<T*>(p.out) + (long)(t.x + t.z + row) * p.o_stride + (long)t.w * W;
 #pragma unroll
-        for (int c = 0; c < D; c += 16) {
-          uint32_t w[8];
+      for (int c = 0; c < W; c += 32) {
+        float o[32];
+        combine(c, o);
+        if (c + 32 == W) {  // all read: the next tile's values may come
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(o_empty);
+        }
+        if (p.norm_w) {
 #pragma unroll
-          for (int e = 0; e < 8; e++) w[e] = pack2<T>(o[c + 2 * e], o[c + 2 * e + 1]);
-          store32(out + c, w, wide);
+          for (int e = 0; e < 32; e += 4) {
+            const float4 w = nw[(c + e) / 4];
+            o[e] *= f * w.x, o[e + 1] *= f * w.y, o[e + 2] *= f * w.z, o[e + 3] *= f * w.w;
+          }
+        }
+        if (t.z + row < t.y) {
+#pragma unroll
+          for (int h = 0; h < 32; h += 16) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = pack2<T>(o[h + 2 * e], o[h + 2 * e + 1]);
+            store32(out + c + h, w, wide);
+          }
         }
       }
       n++;
