@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(WARPS * 32) diff_mma_kernel(DiffParams p) {
   constexpr int W = 2 * D, TILE = 64 * W * 2;
   if (blockIdx.x == 0 && blockIdx.y == 0) check_offsets(p, WARPS * 32);
   Where wh;
-  if (!find_block(p, blockIdx.x, BQ, wh) || wh.len < p.min_len || wh.len > p.max_len) return;
+  if (!find_block(p, p.offsets, blockIdx.x, BQ, wh) || wh.len < p.min_len || wh.len > p.max_len) return;
   extern __shared__ __align__(128) uint8_t smem_diff[];
   const uint32_t sq = (uint32_t)__cvta_generic_to_shared(smem_diff), skv = sq + TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;

@@ -17,22 +17,22 @@ struct Where {
   int t0, len, q0;  // first row and length of the sequence, first query of the block
 };
 
-// The sequence of block number `tile`, found by the calling warp (32 probes a
-// step).  False when the block is empty or the offsets do not describe
+// The sequence of block number `tile` in `offsets` (p.offsets or a copy), found
+// by the calling warp (32 probes a step).  False when the block is empty or the offsets do not describe
 // sequences within [0, T] (reported).
-__device__ __forceinline__ bool find_block(const DiffParams& p, int tile, int bq, Where& w) {
+__device__ __forceinline__ bool find_block(const DiffParams& p, const int32_t* offsets, int tile, int bq, Where& w) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = p.nseq;  // the answer is in [lo, hi)
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32;
     const int i = lo + lane * step;
-    const bool le = i < hi && (long)p.offsets[i] / bq + i <= tile;
+    const bool le = i < hi && (long)offsets[i] / bq + i <= tile;
     const int n = __popc(__ballot_sync(0xffffffffu, le));
     if (n == 0) return false;
     lo += (n - 1) * step;
     hi = min(hi, lo + step);
   }
-  const int t0 = p.offsets[lo], t1 = p.offsets[lo + 1];
+  const int t0 = offsets[lo], t1 = offsets[lo + 1];
   if (t0 < 0 || t1 < t0 || t1 > p.T) {
     if (lane == 0) report(p.status, DE_BOUNDS, 80, lo);
     return false;

@@ -53,7 +53,9 @@ constexpr int BQ = 128, BKEY = 64;
 constexpr int QTILE = 128 * 128, KTILE = 64 * 128;  // bytes of 128 and 64 rows x 64 columns
 constexpr int KV = 4;                               // stages of K and of V
 constexpr int NTHREADS = 512;
-constexpr int RING = 1;
+constexpr int RING = 4;
+constexpr int AHEAD = 8;    // tiles of more key blocks are taken one at a time
+constexpr int OFFS = 1024;  // sequences whose offsets are copied to shared memory
 constexpr float GROW = 8.f;  // log2 of the growth that moves the maximum
 
 template <int D>
@@ -66,8 +68,10 @@ struct Lay {
   static constexpr int OFF_V = OFF_K + KV * KB;  // [KV]
   static constexpr int OFF_L = OFF_V + KV * KB;  // sums [2 tiles][2 maps][128]
   static constexpr int OFF_RING = OFF_L + 2 * 2 * 128 * 4;
-  static constexpr int OFF_NORM = OFF_RING + RING * 16 + 16;  // the next item's answer; norm weights [2d]
-  static constexpr int OFF_BAR = OFF_NORM + 2 * D * 4;
+  static constexpr int OFF_ITEM = OFF_RING + RING * 16;  // the answer that holds the next item
+  static constexpr int OFF_NORM = OFF_ITEM + 16;         // norm weights [2d]
+  static constexpr int OFF_OFFS = OFF_NORM + 2 * D * 4;
+  static constexpr int OFF_BAR = OFF_OFFS + (OFFS + 2) * 4;
   // q_full q_empty [2 each], k_full k_empty v_full v_empty [KV each], s_full
   // p_full [2 maps][2], o_done [2], o_full o_empty sum_full v_fixed, ring_full
   // ring_empty [RING], turn [2 maps][4 quarters], next item
@@ -228,23 +232,23 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         return true;
       };
       auto ring_free = [&]() -> bool {  // every reader has taken the last tile
-        return __all_sync(0xffffffffu,
-                          mbar_wait(ring_empty(n % RING), ((n / RING) & 1) ^ 1, abort_flag, status, 82)) != 0;
+        return __all_sync(0xffffffffu, mbar_wait(ring_empty((n - 1) % RING), ((n - 1) / RING) & 1, abort_flag, status,
+                                                 82)) != 0;
       };
+      const int32_t* offsets = p.offsets;
+      if (p.nseq <= OFFS) {
+        int32_t* copy = reinterpret_cast<int32_t*>(smem + L::OFF_OFFS);
+        for (int s = lane; s <= p.nseq; s += 32) copy[s] = p.offsets[s];
+        __syncwarp();
+        offsets = copy;
+      }
       // The first item is the CTA's own; further ones are CTAs of the grid that
       // have not started, cancelled one at a time, so that the items go to
-      // whichever SM is free.
-      const uint32_t answer = sbase + L::OFF_RING + RING * 16;
-      Where w{};
-      int last = -1;
-      bool found = false, ok = true;
-      uint32_t item = blockIdx.x;
-      for (uint32_t k = 0;; k++) {
-        const int tile = (int)(item / (uint32_t)p.heads), head = (int)(item - (uint32_t)tile * p.heads);
-        if (tile != last) found = find_block(p, tile, BQ, w) && w.len >= p.min_len;
-        last = tile;
-        if (found) ok = publish(make_int4(w.t0, w.len, w.q0, head)) && ring_free();
-        if (!ok) break;
+      // whichever SM is free.  The next is asked for while this one is looked
+      // up, but behind a long tile only when every reader has taken it: what
+      // a CTA holds, no other can do.
+      const uint32_t answer = sbase + L::OFF_ITEM;
+      auto ask = [&]() {
         if (lane == 0) {
           mbar_expect_tx(item_bar, 16);
           asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::
@@ -253,6 +257,23 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                        : "memory");
         }
         __syncwarp();
+      };
+      Where w{};
+      int last = -1;
+      bool found = false, ok = true, asked = false;
+      uint32_t item = blockIdx.x;
+      for (uint32_t k = 0;; k++) {
+        const int tile = (int)(item / (uint32_t)p.heads), head = (int)(item - (uint32_t)tile * p.heads);
+        if (tile != last) found = find_block(p, offsets, tile, BQ, w) && w.len >= p.min_len;
+        last = tile;
+        asked = !found || w.len <= AHEAD * BKEY;
+        if (asked) ask();
+        if (found) ok = publish(make_int4(w.t0, w.len, w.q0, head));
+        if (!asked) {
+          ok = ok && ring_free();
+          if (ok) ask();
+        }
+        if (!ok) break;
         ok = __all_sync(0xffffffffu, mbar_wait(item_bar, k & 1, abort_flag, status, 81));
         if (!ok) break;
         uint64_t lo, hi;
