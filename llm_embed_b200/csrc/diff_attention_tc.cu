@@ -66,17 +66,18 @@ struct Lay {
   static constexpr int OFF_Q = 0;         // [2]
   static constexpr int OFF_K = 2 * QB;    // [KV]
   static constexpr int OFF_V = OFF_K + KV * KB;  // [KV]
-  static constexpr int OFF_L = OFF_V + KV * KB;  // sums [2 tiles][2 maps][128]
+  static constexpr int OFF_OUT = OFF_V + KV * KB;  // results on their way out [4 warps][32 rows][64]
+  static constexpr int OFF_L = OFF_OUT + 4 * 4096;  // sums [2 tiles][2 maps][128]
   static constexpr int OFF_RING = OFF_L + 2 * 2 * 128 * 4;
   static constexpr int OFF_ITEM = OFF_RING + RING * 16;  // the answer that holds the next item
   static constexpr int OFF_NORM = OFF_ITEM + 16;         // norm weights [2d]
   static constexpr int OFF_OFFS = OFF_NORM + 2 * D * 4;
   static constexpr int OFF_BAR = OFF_OFFS + (OFFS + 2) * 4;
   // q_full q_empty [2 each], k_full k_empty v_full v_empty [KV each], s_full
-  // p_full [2 maps][2], o_done [2], o_full o_empty sum_full v_fixed, ring_full
-  // ring_empty [RING], turn [2 maps][4 quarters], next item
+  // p_full [2 maps][2], o_done [2], o_full o_empty, sum_full sum_empty [2 each],
+  // ring_full ring_empty [RING], turn [2 maps][4 quarters], next item
   static constexpr int B_Q = 0, B_K = 4, B_V = B_K + 2 * KV, B_S = B_V + 2 * KV, B_P = B_S + 4, B_D = B_P + 4,
-                       B_O = B_D + 2, B_R = B_O + 4, B_T = B_R + 2 * RING, NBAR = B_T + 9;
+                       B_O = B_D + 2, B_R = B_O + 6, B_T = B_R + 2 * RING, NBAR = B_T + 9;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;
   static_assert(ALLOC <= 232448, "shared memory of one CTA");
@@ -90,6 +91,13 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -114,22 +122,10 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
   return e != 0;
 }
-// 32 bytes of a row.
-__device__ __forceinline__ void store32(void* p, const uint32_t* w, bool wide) {
-  if (wide) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-  } else {
-    static_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-  }
-}
-
 template <class T, int D>
 __global__ void __launch_bounds__(NTHREADS, 1)
     diff_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                   const __grid_constant__ CUtensorMap tmap_v, DiffParams p, int wide) {
+                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_o, DiffParams p) {
   using L = Lay<D>;
   constexpr int NT = L::NT, W = 2 * D;
   constexpr uint32_t FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0;
@@ -148,7 +144,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   auto s_full = [&](int i, uint32_t b) { return bar0 + 8 * (L::B_S + 2 * i + (b & 1)); };
   auto p_full = [&](int i, uint32_t b) { return bar0 + 8 * (L::B_P + 2 * i + (b & 1)); };
   auto o_done = [&](int i) { return bar0 + 8 * (L::B_D + i); };
-  const uint32_t o_full = bar0 + 8 * L::B_O, o_empty = o_full + 8, sum_full = o_full + 16, v_fixed = o_full + 24;
+  const uint32_t o_full = bar0 + 8 * L::B_O, o_empty = o_full + 8;
+  auto sum_full = [&](uint32_t n) { return bar0 + 8 * (L::B_O + 2 + (n & 1)); };
+  auto sum_empty = [&](uint32_t n) { return bar0 + 8 * (L::B_O + 4 + (n & 1)); };
   auto ring_full = [&](int e) { return bar0 + 8 * (L::B_R + e); };
   auto ring_empty = [&](int e) { return bar0 + 8 * (L::B_R + RING + e); };
   auto turn = [&](int i, int q) { return bar0 + 8 * (L::B_T + 4 * i + q); };
@@ -177,10 +175,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       mbar_init(v_empty(s), 2);
     }
     mbar_init(o_full, 2);
-    mbar_init(v_fixed, 4);
     for (int i = 0; i < 9; i++) mbar_init(turn(0, i), 1);  // and item_bar
     mbar_init(o_empty, 4);
-    mbar_init(sum_full, 8);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(sum_full(i), 8);
+      mbar_init(sum_empty(i), 4);
+    }
     for (int e = 0; e < RING; e++) {
       mbar_init(ring_full(e), 1);
       mbar_init(ring_empty(e), 15);  // producer, two MMA, eight softmax, four epilogue warps
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   };
 
   // 512 threads of 128 registers at launch; the softmax threads take what the
-  // others leave: 56 + 2 * 176 + 104 = 4 * 128.
+  // others leave, as do the epilogue's: 56 + 2 * 144 + 168 = 4 * 128.
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 3) {
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const int i = warp - 1;  // map
       const bool issuer = elect_one();
       const uint32_t s_tm = tmem + i * 128, o_tm = tmem + TM_O + i * W;
-      uint32_t n = 0, ib = 0, fixed = 0;
+      uint32_t n = 0, ib = 0;
       int4 t;
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity, int site) {
@@ -365,7 +365,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         for (int j = 0; j < nkb; j++, ib++) {
           const int left = t.y - j * BKEY, steps = min(BKEY, left + 15) / 16;
           if (!wait(v_full(ib % KV), (ib / KV) & 1, 67)) break;
-          if (left < BKEY && left % 16 != 0 && !wait(v_fixed, fixed++ & 1, 69)) break;
           if (!wait(p_full(i, ib), (ib >> 1) & 1, 73)) break;
           tc_fence_after();
           if (issuer) {
@@ -393,7 +392,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
     }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     // -------------------------------------------------------------- softmax
     const int map = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -494,8 +493,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         float a, b;
         f2_unpack(f2_add(s0, s1), a, b);
         l += a + b;
-        if (map == 0 && left < BKEY && left % 16 != 0) {
-          // The values between the last key and the end of its 16.
+        if (left < BKEY && left % 16 != 0) {
+          // The values between the last key and the end of its 16 (both maps'
+          // threads write the same zeros, each before its own product).
           ok = __all_sync(0xffffffffu, mbar_wait(v_full(ib % KV), (ib / KV) & 1, abort_flag, status, 75));
           if (!ok) break;
           const int rows = 16 - left % 16;
@@ -503,8 +503,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           for (int e = row; e < rows * 8 * NT; e += 128)
             *reinterpret_cast<uint4*>(v + e / (rows * 8) * KTILE + e % (rows * 8) * 16) = make_uint4(0, 0, 0, 0);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(v_fixed);
         }
         wait_st();
         tc_fence_before();
@@ -512,81 +510,90 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (lane == 0) mbar_arrive(p_full(map, ib));
       }
       if (!ok) break;
-      // The row's sum, for the epilogue (two buffers: it has read a tile's
-      // before the next one's results can be complete).
+      // The row's sum, for the epilogue: two buffers, since the softmax of short
+      // tiles runs ahead of the results.
+      ok = __all_sync(0xffffffffu, mbar_wait(sum_empty(n), ((n >> 1) & 1) ^ 1, abort_flag, status, 78));
+      if (!ok) break;
       sums[(n & 1) * 256 + map * 128 + row] = l;
       __syncwarp();
-      if (lane == 0) mbar_arrive(sum_full);
+      if (lane == 0) mbar_arrive(sum_full(n));
       n++;
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ------------------------------------------------------------- epilogue
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t o1 = tmem + TM_O + ((uint32_t)(quarter * 32) << 16);
     const float* sums = reinterpret_cast<const float*>(smem + L::OFF_L);
     const float4* nw = reinterpret_cast<const float4*>(smem + L::OFF_NORM);
+    const uint32_t stage = sbase + L::OFF_OUT + quarter * 4096;
     uint32_t n = 0;
     int4 t;
     while (next_tile(n, t)) {
       const float lambda = p.lambda[t.w];
-      if (!__all_sync(0xffffffffu, mbar_wait(sum_full, n & 1, abort_flag, status, 77)) ||
+      if (!__all_sync(0xffffffffu, mbar_wait(sum_full(n), (n >> 1) & 1, abort_flag, status, 77)) ||
           !__all_sync(0xffffffffu, mbar_wait(o_full, n & 1, abort_flag, status, 76)))
         break;
       tc_fence_after();
       const float* sum = sums + (n & 1) * 256;
       const float w1 = 1.f / sum[row], w2 = -lambda / sum[128 + row];
-      // o of 32 columns; a second look at them costs less than the registers
-      // that would keep them.
-      auto combine = [&](int c, float (&o)[32]) {
-        uint32_t a[32], b[32];
-        ld32(o1 + c, a);
-        ld32(o1 + W + c, b);
+      float o[W], ss = 0.f;
+#pragma unroll
+      for (int c = 0; c < W; c += 16) {
+        uint32_t a[16], b[16];
+        ld16(o1 + c, a);
+        ld16(o1 + W + c, b);
         wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; e++) o[e] = fmaf(__uint_as_float(a[e]), w1, __uint_as_float(b[e]) * w2);
-      };
-      float f = 1.f;
-      if (p.norm_w) {
-        float ss = 0.f;
-#pragma unroll
-        for (int c = 0; c < W; c += 32) {
-          float o[32];
-          combine(c, o);
-#pragma unroll
-          for (int e = 0; e < 32; e++) ss = fmaf(o[e], o[e], ss);
+        for (int e = 0; e < 16; e++) {
+          o[c + e] = fmaf(__uint_as_float(a[e]), w1, __uint_as_float(b[e]) * w2);
+          ss = fmaf(o[c + e], o[c + e], ss);
         }
-        f = p.out_scale * rsqrtf(ss * (1.f / W) + p.eps);
       }
-      T* out = static_cast<T*>(p.out) + (long)(t.x + t.z + row) * p.o_stride + (long)t.w * W;
+      tc_fence_before();  // all read: the next tile's values may come
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(o_empty);
+        mbar_arrive(sum_empty(n));
+      }
+      if (p.norm_w) {
+        const float f = p.out_scale * rsqrtf(ss * (1.f / W) + p.eps);
 #pragma unroll
-      for (int c = 0; c < W; c += 32) {
-        float o[32];
-        combine(c, o);
-        if (c + 32 == W) {  // all read: the next tile's values may come
-          tc_fence_before();
+        for (int c = 0; c < W; c += 4) {
+          const float4 w = nw[c / 4];
+          o[c] *= f * w.x, o[c + 1] *= f * w.y, o[c + 2] *= f * w.z, o[c + 3] *= f * w.w;
+        }
+      }
+      // 64 columns at a time; a warp whose 32 rows are all the sequence's
+      // stores them through shared memory with TMA, others row by row.
+      const bool whole = t.z + quarter * 32 + 32 <= t.y;
+#pragma unroll
+      for (int c = 0; c < W; c += 64) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; e++) w[e] = pack2<T>(o[c + 2 * e], o[c + 2 * e + 1]);
+        if (whole) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(o_empty);
-        }
-        if (p.norm_w) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 w = nw[(c + e) / 4];
-            o[e] *= f * w.x, o[e + 1] *= f * w.y, o[e + 2] *= f * w.z, o[e + 3] *= f * w.w;
-          }
-        }
-        if (t.z + row < t.y) {
+          for (int q = 0; q < 8; q++)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((q ^ (lane & 7)) << 4)),
+                         "r"(w[4 * q]), "r"(w[4 * q + 1]), "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
+                         : "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) tma_store_2d(&tmap_o, stage, t.w * W + c, t.x + t.z + quarter * 32);
+        } else if (t.z + row < t.y) {
+          uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (long)(t.x + t.z + row) * p.o_stride +
+                                                (long)t.w * W + c);
 #pragma unroll
-          for (int h = 0; h < 32; h += 16) {
-            uint32_t w[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) w[e] = pack2<T>(o[h + 2 * e], o[h + 2 * e + 1]);
-            store32(out + c + h, w, wide);
-          }
+          for (int q = 0; q < 8; q++) out[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
         }
       }
       n++;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -627,9 +634,10 @@ static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   const int kvh = p.heads / p.group;
-  if (!encode(&mq, p.q, p.heads, p.q_stride, BQ) || !encode(&mk, p.k, kvh, p.k_stride, BKEY) || !encode(&mv, p.v, kvh, p.v_stride, BKEY))
+  if (!encode(&mq, p.q, p.heads, p.q_stride, BQ) || !encode(&mk, p.k, kvh, p.k_stride, BKEY) || !encode(&mv, p.v, kvh, p.v_stride, BKEY) ||
+      !encode(&mo, p.out, p.heads, p.o_stride, 32))
     return cudaErrorInvalidValue;
   static std::mutex mu;
   static uint64_t attr_set = 0;  // per-device bit: the attribute is a per-device setting
@@ -647,11 +655,10 @@ static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
   const int tiles = block_count(p.T, p.nseq, BQ);
   const long items = (long)tiles * p.heads;
   if (items > 0x7fffffff) return cudaErrorInvalidValue;
-  const int wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.o_stride % 16 == 0;
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)items), dim3(NTHREADS),
                                             Lay<D>::ALLOC, s, attr);
-  return cudaLaunchKernelEx(&cfg, diff_tc_kernel<T, D>, mq, mk, mv, p, wide);
+  return cudaLaunchKernelEx(&cfg, diff_tc_kernel<T, D>, mq, mk, mv, mo, p);
 }
 
 }  // namespace dtc

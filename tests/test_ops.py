@@ -659,6 +659,34 @@ def test_diff_attention(lens, h, hkv, d, name, norm):
 
 
 @gpu
+@pytest.mark.parametrize("count,lo,hi", [(700, 1, 64), (700, 16, 128), (700, 65, 100), (700, 1, 300), (3000, 0, 9)])
+@pytest.mark.parametrize("norm", [True, False])
+def test_diff_attention_many_sequences(count, lo, hi, norm):
+    """Many tiles per SM, short ones among them: the steps of a tile overlap
+    those of the next ones, and twice gives the same bits."""
+    import torch
+    h, d = 6, 64
+    lens = np.random.default_rng(hi).integers(lo, hi + 1, count).tolist()
+    q, k, v, offs, t = make_diff(lens, h, h, d, "f16", hi)
+    lam, val = lambdas(h, d, True, 3)
+    nw = (1 + 0.3 * torch.randn(2 * d, generator=torch.Generator().manual_seed(1))) if norm else None
+    a = ops.DiffAttention(h, h, d, lam, INIT, None if nw is None else nw.numpy(), 1e-5)
+    for hint in (0, hi):
+        out = run_diff(a, q, k, v, offs, t, h, d, "f16", hint)
+        for _ in range(3):
+            assert torch.equal(out, run_diff(a, q, k, v, offs, t, h, d, "f16", hint))
+        a.sync()
+        part = torch.arange(0, count, 23).tolist()
+        for s in part:
+            x, y = int(offs[s]), int(offs[s + 1])
+            if x == y:
+                continue
+            ref, mag = diff64(q[x:y], k[x:y], v[x:y], [0, y - x], h, h, d, val, INIT, None if nw is None else nw.cuda(), 1e-5)
+            check_diff(out[x:y], ref, mag, "f16")
+    a.close()
+
+
+@gpu
 @pytest.mark.parametrize("lens", [[5], [60, 70], [200, 130], [600]])
 @pytest.mark.parametrize("name", ["f16", "bf16"])
 def test_diff_attention_ignores_other_rows(lens, name):
