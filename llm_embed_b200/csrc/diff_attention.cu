@@ -5,12 +5,15 @@
 // for every head, whose two query and key parts have d columns each and whose
 // values have 2d.
 //
-// A CTA has 64 queries of one head and sequence, 16 per warp, and goes once
-// over the keys in blocks of 64, two in flight (cp.async).  Each map keeps a
-// running maximum and sum per query and its own float32 result O_i, rescaled
-// when the maximum grows; at the end o = O_1 / l_1 - lambda O_2 / l_2.  A block's values are read
-// from shared memory once for both maps.  Weights P are rounded to the
-// operands' type (16 bits) for the second product, their sums are not.
+// For sequences of at most 64 tokens, where a call is bound by latency and by
+// how many of them are in flight: a CTA of four warps holds 64 rows of Q, K and
+// V, which are one head of up to 64 tokens, two of up to 32 or four of up to
+// 16; a warp has 16 query rows.  Both maps' scores stay in registers, so the
+// maxima and sums are known before the second product, and it runs once, on
+// P = P_1 / l_1 - lambda P_2 / l_2, rounded to the operands' type (16 bits); the
+// sums are not.  Longer sequences (a caller whose hint of the longest was too
+// small) take the same steps block by block, in two passes: maxima and sums,
+// then weights and values.
 // Keys past the sequence get weight 0 and their values are zeros in shared
 // memory, whatever the rows behind hold.
 #include <mutex>
@@ -56,193 +59,256 @@ __device__ __forceinline__ uint32_t at(uint32_t base, int row, int chunk) {
   return base + row * (W * 2) + ((chunk ^ (row & 7)) << 4);
 }
 
-// Rows [0, 64) of a tile from src (row stride ld); rows from `n` on are zero.
+// 64 rows of a tile: row r is token r % per of head r / per, from src + token *
+// ld + head * W; tokens from `n` on and heads from `heads` on are zero.  GROUP
+// query heads share a head of src.
 template <int W, class T>
-__device__ __forceinline__ void load_tile(uint32_t base, const T* src, long ld, int n) {
+__device__ __forceinline__ void load_tile(uint32_t base, const T* src, long ld, int per, int n, int head0, int heads,
+                                          int group) {
   constexpr int CH = W / 8;
 #pragma unroll
-  for (int i = threadIdx.x; i < 64 * CH; i += WARPS * 32) {
-    const int r = i / CH, c = i % CH;
-    const int bytes = r < n ? 16 : 0;
-    const T* g = src + (long)(r < n ? r : 0) * ld + c * 8;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at<W>(base, r, c)), "l"(g), "r"(bytes));
+  for (int k = 0; k < 64 * CH / (WARPS * 32); k++) {
+    const int i = k * (WARPS * 32) + threadIdx.x, r = i / CH, c = i % CH;
+    const int token = r & (per - 1), head = head0 + r / per;
+    const bool in = token < n && head < heads;
+    const T* g = src + (long)(in ? token : 0) * ld + (long)((in ? head : head0) / group) * W + c * 8;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at<W>(base, r, c)), "l"(g), "r"(in ? 16 : 0));
+  }
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// Scores of a warp's 16 rows against keys key0 .. key0 + 63 of a tile (those of
+// the first `left`; -inf behind), for part `i` of the head.
+template <class T, int D>
+__device__ __forceinline__ void scores(float (&s)[8][4], uint32_t sq, uint32_t sk, int i, int row0, int key0, int left) {
+  constexpr int W = 2 * D;
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  uint32_t qa[D / 16][4];
+#pragma unroll
+  for (int c = 0; c < D / 16; c++) ldsm4(qa[c], at<W>(sq, row0 + (lane & 15), i * (D / 8) + 2 * c + (lane >> 4)));
+#pragma unroll
+  for (int n = 0; n < 8; n++) {
+    s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    if (n * 8 < left) {
+#pragma unroll
+      for (int c = 0; c < D / 16; c += 2) {
+        uint32_t b[4];
+        ldsm4(b, at<W>(sk, key0 + n * 8 + (lane & 7), i * (D / 8) + 2 * c + (lane >> 3)));
+        mma16<T>(s[n], qa[c], b[0], b[1]);
+        mma16<T>(s[n], qa[c + 1], b[2], b[3]);
+      }
+    }
+    if (n * 8 + 8 > left) {
+      const int key = n * 8 + 2 * t;
+      if (key >= left) s[n][0] = s[n][2] = -INFINITY;
+      if (key + 1 >= left) s[n][1] = s[n][3] = -INFINITY;
+    }
   }
 }
 
+// A row pair's running maximum and sum of one map.
+struct Stat {
+  float m[2], l[2];
+};
+
+// The block's part of the statistics; s becomes exp2(scale (s - m)).
+__device__ __forceinline__ void add_block(Stat& st, float (&s)[8][4], float scale) {
+  float m0 = st.m[0], m1 = st.m[1];
+#pragma unroll
+  for (int n = 0; n < 8; n++) {
+    m0 = fmaxf(m0, fmaxf(s[n][0], s[n][1]));
+    m1 = fmaxf(m1, fmaxf(s[n][2], s[n][3]));
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+  }
+  float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int n = 0; n < 8; n++) {
+    s[n][0] = ex2f(fmaf(s[n][0], scale, -m0 * scale));
+    s[n][1] = ex2f(fmaf(s[n][1], scale, -m0 * scale));
+    s[n][2] = ex2f(fmaf(s[n][2], scale, -m1 * scale));
+    s[n][3] = ex2f(fmaf(s[n][3], scale, -m1 * scale));
+    l0 += s[n][0] + s[n][1];
+    l1 += s[n][2] + s[n][3];
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+  }
+  st.l[0] = fmaf(st.l[0], ex2f((st.m[0] - m0) * scale), l0);
+  st.l[1] = fmaf(st.l[1], ex2f((st.m[1] - m1) * scale), l1);
+  st.m[0] = m0;
+  st.m[1] = m1;
+}
+
+// o += P V for the weights w1 a - w2 b of the first `left` keys from key0.
+template <class T, int W>
+__device__ __forceinline__ void values(float (&o)[W / 8][4], const float (&a)[8][4], const float (&b)[8][4],
+                                       const float (&w1)[2], const float (&w2)[2], uint32_t sv, int key0, int left) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < BKEY / 16; c++)
+    if (c * 16 < left) {
+      uint32_t pa[4];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int n = 2 * c + h;
+        pa[2 * h] = pack2<T>(fmaf(a[n][0], w1[0], -b[n][0] * w2[0]), fmaf(a[n][1], w1[0], -b[n][1] * w2[0]));
+        pa[2 * h + 1] = pack2<T>(fmaf(a[n][2], w1[1], -b[n][2] * w2[1]), fmaf(a[n][3], w1[1], -b[n][3] * w2[1]));
+      }
+#pragma unroll
+      for (int n = 0; n < W / 8; n += 2) {
+        uint32_t f[4];
+        ldsm4_t(f, at<W>(sv, key0 + c * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, n + (lane >> 4)));
+        mma16<T>(o[n], pa, f[0], f[1]);
+        mma16<T>(o[n + 1], pa, f[2], f[3]);
+      }
+    }
+}
+
 template <class T, int D>
-__global__ void __launch_bounds__(WARPS * 32) diff_mma_kernel(DiffParams p) {
+__global__ void __launch_bounds__(WARPS * 32, 3) diff_short_kernel(DiffParams p) {
+  constexpr int W = 2 * D, TILE = 64 * W * 2;
   pdl_wait();
   pdl_trigger();
-  constexpr int W = 2 * D, TILE = 64 * W * 2;
   if (blockIdx.x == 0 && blockIdx.y == 0) check_offsets(p, WARPS * 32);
   Where wh;
   if (!find_block(p, p.offsets, blockIdx.x, BQ, wh) || wh.len < p.min_len || wh.len > p.max_len) return;
+  const int per = wh.len <= 16 ? 16 : wh.len <= 32 ? 32 : 64;  // rows of a head in the tiles
+  const int head0 = blockIdx.y * (64 / per);
+  if (head0 >= p.heads) return;
   extern __shared__ __align__(128) uint8_t smem_diff[];
-  const uint32_t sq = (uint32_t)__cvta_generic_to_shared(smem_diff), skv = sq + TILE;
+  const uint32_t sq = (uint32_t)__cvta_generic_to_shared(smem_diff), sk = sq + TILE, sv = sk + TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int head = blockIdx.y, kvh = head / p.group;
-  const T* q = static_cast<const T*>(p.q) + (long)(wh.t0 + wh.q0) * p.q_stride + (long)head * W;
-  const T* k = static_cast<const T*>(p.k) + (long)wh.t0 * p.k_stride + (long)kvh * W;
-  const T* v = static_cast<const T*>(p.v) + (long)wh.t0 * p.v_stride + (long)kvh * W;
-  const int nkb = (wh.len + BKEY - 1) / BKEY;
-  auto load_kv = [&](int j) {
-    const uint32_t b = skv + (j & 1) * 2 * TILE;
-    load_tile<W>(b, k + (long)j * BKEY * p.k_stride, p.k_stride, wh.len - j * BKEY);
-    load_tile<W>(b + TILE, v + (long)j * BKEY * p.v_stride, p.v_stride, wh.len - j * BKEY);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  load_tile<W>(sq, q, p.q_stride, wh.len - wh.q0);
-  load_kv(0);
+  const int row0 = warp * 16, key0 = row0 & ~(per - 1);      // in the tiles
+  const int head = head0 + row0 / per, first = wh.q0 + (row0 & (per - 1));  // the warp's head and first token
+  const bool work = head < p.heads && first < wh.len;        // warp-uniform
+  const T* q = static_cast<const T*>(p.q) + (long)(wh.t0 + wh.q0) * p.q_stride;
+  const T* k = static_cast<const T*>(p.k) + (long)wh.t0 * p.k_stride;
+  const T* v = static_cast<const T*>(p.v) + (long)wh.t0 * p.v_stride;
+  const float scale = 1.4426950408889634f * rsqrtf((float)D);
+  const float lambda = work ? p.lambda[head] : 0.f;
+  float o[W / 8][4];
+#pragma unroll
+  for (int n = 0; n < W / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
-  uint32_t qa[2][D / 16][4];
-  float o[2][W / 8][4], m[2][2], l[2][2];
+  load_tile<W>(sq, q, p.q_stride, per, wh.len - wh.q0, head0, p.heads, 1);
+  Stat st[2];
 #pragma unroll
   for (int i = 0; i < 2; i++) {
-    m[i][0] = m[i][1] = -INFINITY;
-    l[i][0] = l[i][1] = 0.f;
-#pragma unroll
-    for (int n = 0; n < W / 8; n++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+    st[i].m[0] = st[i].m[1] = -INFINITY;
+    st[i].l[0] = st[i].l[1] = 0.f;
   }
-  const float scale2 = 1.4426950408889634f * rsqrtf((float)D);
-  for (int j = 0; j < nkb; j++) {
-    if (j + 1 < nkb) {
-      load_kv(j + 1);
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-    } else {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-    }
+  if (wh.len <= BKEY) {
+    load_tile<W>(sk, k, p.k_stride, per, wh.len, head0, p.heads, p.group);
+    commit_copies();
+    load_tile<W>(sv, v, p.v_stride, per, wh.len, head0, p.heads, p.group);
+    commit_copies();
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncthreads();
-    if (j == 0) {
+    float s[2][8][4];
+    if (work) {
 #pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int c = 0; c < D / 16; c++)
-          ldsm4(qa[i][c], at<W>(sq, warp * 16 + (lane & 15), i * (D / 8) + 2 * c + (lane >> 4)));
-    }
-    const uint32_t sk = skv + (j & 1) * 2 * TILE, sv = sk + TILE;
-    const int left = wh.len - j * BKEY;  // keys of this block and behind
-    uint32_t pa[2][BKEY / 16][4];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      float s[BKEY / 8][4];
-#pragma unroll
-      for (int n = 0; n < BKEY / 8; n++) {
-        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-        for (int c = 0; c < D / 16; c += 2) {
-          uint32_t b[4];
-          ldsm4(b, at<W>(sk, n * 8 + (lane & 7), i * (D / 8) + 2 * c + (lane >> 3)));
-          mma16<T>(s[n], qa[i][c], b[0], b[1]);
-          mma16<T>(s[n], qa[i][c + 1], b[2], b[3]);
-        }
-      }
-      float mx0 = m[i][0], mx1 = m[i][1];
-#pragma unroll
-      for (int n = 0; n < BKEY / 8; n++) {
-        if (left < BKEY) {
-          const int key = n * 8 + 2 * t;
-          if (key >= left) s[n][0] = s[n][2] = -INFINITY;
-          if (key + 1 >= left) s[n][1] = s[n][3] = -INFINITY;
-        }
-        mx0 = fmaxf(mx0, fmaxf(s[n][0], s[n][1]));
-        mx1 = fmaxf(mx1, fmaxf(s[n][2], s[n][3]));
-      }
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-      const float c0 = ex2f((m[i][0] - mx0) * scale2), c1 = ex2f((m[i][1] - mx1) * scale2);
-      m[i][0] = mx0;
-      m[i][1] = mx1;
-      const float off0 = -mx0 * scale2, off1 = -mx1 * scale2;
-      float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-      for (int n = 0; n < BKEY / 8; n++) {
-        s[n][0] = ex2f(fmaf(s[n][0], scale2, off0));
-        s[n][1] = ex2f(fmaf(s[n][1], scale2, off0));
-        s[n][2] = ex2f(fmaf(s[n][2], scale2, off1));
-        s[n][3] = ex2f(fmaf(s[n][3], scale2, off1));
-        l0 += s[n][0] + s[n][1];
-        l1 += s[n][2] + s[n][3];
-      }
-      l[i][0] = fmaf(l[i][0], c0, l0);
-      l[i][1] = fmaf(l[i][1], c1, l1);
-#pragma unroll
-      for (int n = 0; n < W / 8; n++) {
-        o[i][n][0] *= c0;
-        o[i][n][1] *= c0;
-        o[i][n][2] *= c1;
-        o[i][n][3] *= c1;
-      }
-#pragma unroll
-      for (int n = 0; n < BKEY / 16; n++) {
-        pa[i][n][0] = pack2<T>(s[2 * n][0], s[2 * n][1]);
-        pa[i][n][1] = pack2<T>(s[2 * n][2], s[2 * n][3]);
-        pa[i][n][2] = pack2<T>(s[2 * n + 1][0], s[2 * n + 1][1]);
-        pa[i][n][3] = pack2<T>(s[2 * n + 1][2], s[2 * n + 1][3]);
+      for (int i = 0; i < 2; i++) {
+        scores<T, D>(s[i], sq, sk, i, row0, key0, wh.len);
+        add_block(st[i], s[i], scale);
       }
     }
-#pragma unroll
-    for (int c = 0; c < BKEY / 16; c++)
-#pragma unroll
-      for (int n = 0; n < W / 8; n += 2) {
-        uint32_t b[4];
-        ldsm4_t(b, at<W>(sv, c * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, n + (lane >> 4)));
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          mma16<T>(o[i][n], pa[i][c], b[0], b[1]);
-          mma16<T>(o[i][n + 1], pa[i][c], b[2], b[3]);
-        }
-      }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
+    if (!work) return;
+    const float w1[2] = {1.f / st[0].l[0], 1.f / st[0].l[1]};
+    const float w2[2] = {lambda / st[1].l[0], lambda / st[1].l[1]};
+    values<T, W>(o, s[0], s[1], w1, w2, sv, key0, wh.len);
+  } else {
+    for (int pass = 0; pass < 2; pass++) {
+      float w1[2], w2[2];
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        w1[r] = 1.f / st[0].l[r];
+        w2[r] = lambda / st[1].l[r];
+      }
+      for (int j = 0; j * BKEY < wh.len; j++) {
+        const int left = wh.len - j * BKEY;
+        load_tile<W>(sk, k + (long)j * BKEY * p.k_stride, p.k_stride, per, left, head0, p.heads, p.group);
+        if (pass == 1) load_tile<W>(sv, v + (long)j * BKEY * p.v_stride, p.v_stride, per, left, head0, p.heads, p.group);
+        commit_copies();
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        if (work) {
+          float s[2][8][4];
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            scores<T, D>(s[i], sq, sk, i, row0, 0, left);
+            if (pass == 0) {
+              add_block(st[i], s[i], scale);
+            } else {
+#pragma unroll
+              for (int n = 0; n < 8; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  s[i][n][e] = ex2f(fmaf(s[i][n][e], scale, -st[i].m[e >> 1] * scale));
+            }
+          }
+          if (pass == 1) values<T, W>(o, s[0], s[1], w1, w2, sv, 0, left);
+        }
+        __syncthreads();
+      }
+    }
+    if (!work) return;
   }
 
-  const float lam = p.lambda[head];
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-      l[i][r] += __shfl_xor_sync(0xffffffffu, l[i][r], 1);
-      l[i][r] += __shfl_xor_sync(0xffffffffu, l[i][r], 2);
-    }
-  const float a0 = 1.f / l[0][0], a1 = 1.f / l[0][1], b0 = lam / l[1][0], b1 = lam / l[1][1];
-  float ss0 = 0.f, ss1 = 0.f;
-#pragma unroll
-  for (int n = 0; n < W / 8; n++) {
-#pragma unroll
-    for (int c = 0; c < 2; c++) {
-      o[0][n][c] = o[0][n][c] * a0 - o[1][n][c] * b0;
-      o[0][n][2 + c] = o[0][n][2 + c] * a1 - o[1][n][2 + c] * b1;
-      ss0 = fmaf(o[0][n][c], o[0][n][c], ss0);
-      ss1 = fmaf(o[0][n][2 + c], o[0][n][2 + c], ss1);
-    }
-  }
+  // Norm, then out through the warp's own rows of the query tile: whole
+  // 16-byte chunks of a row instead of pairs of elements.
   float r0 = 1.f, r1 = 1.f;
   if (p.norm_w) {
-    ss0 += __shfl_xor_sync(0xffffffffu, ss0, 1);
-    ss0 += __shfl_xor_sync(0xffffffffu, ss0, 2);
-    ss1 += __shfl_xor_sync(0xffffffffu, ss1, 1);
-    ss1 += __shfl_xor_sync(0xffffffffu, ss1, 2);
+    float ss0 = 0.f, ss1 = 0.f;
+#pragma unroll
+    for (int n = 0; n < W / 8; n++) {
+      ss0 = fmaf(o[n][0], o[n][0], fmaf(o[n][1], o[n][1], ss0));
+      ss1 = fmaf(o[n][2], o[n][2], fmaf(o[n][3], o[n][3], ss1));
+    }
+#pragma unroll
+    for (int e = 1; e < 4; e <<= 1) {
+      ss0 += __shfl_xor_sync(0xffffffffu, ss0, e);
+      ss1 += __shfl_xor_sync(0xffffffffu, ss1, e);
+    }
     r0 = p.out_scale * rsqrtf(ss0 / (float)W + p.eps);
     r1 = p.out_scale * rsqrtf(ss1 / (float)W + p.eps);
   }
-  const int q0 = wh.q0 + warp * 16 + g;
-  T* out = static_cast<T*>(p.out) + (long)(wh.t0 + q0) * p.o_stride + (long)head * W + 2 * t;
+  __syncwarp();
 #pragma unroll
   for (int n = 0; n < W / 8; n++) {
-    const float w0 = p.norm_w ? __ldg(p.norm_w + 8 * n + 2 * t) : 1.f;
-    const float w1 = p.norm_w ? __ldg(p.norm_w + 8 * n + 2 * t + 1) : 1.f;
-    if (q0 < wh.len)
-      *reinterpret_cast<uint32_t*>(out + 8 * n) = pack2<T>(o[0][n][0] * r0 * w0, o[0][n][1] * r0 * w1);
-    if (q0 + 8 < wh.len)
-      *reinterpret_cast<uint32_t*>(out + 8 * p.o_stride + 8 * n) =
-          pack2<T>(o[0][n][2] * r1 * w0, o[0][n][3] * r1 * w1);
+    float2 w = make_float2(1.f, 1.f);
+    if (p.norm_w) w = __ldg(reinterpret_cast<const float2*>(p.norm_w + 8 * n + 2 * t));
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at<W>(sq, row0 + g, n) + 4 * t),
+                 "r"(pack2<T>(o[n][0] * r0 * w.x, o[n][1] * r0 * w.y))
+                 : "memory");
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at<W>(sq, row0 + g + 8, n) + 4 * t),
+                 "r"(pack2<T>(o[n][2] * r1 * w.x, o[n][3] * r1 * w.y))
+                 : "memory");
+  }
+  __syncwarp();
+  T* out = static_cast<T*>(p.out) + (long)(wh.t0 + first) * p.o_stride + (long)head * W;
+#pragma unroll
+  for (int e = lane; e < 16 * (W / 8); e += 32) {
+    const int r = e / (W / 8), c = e % (W / 8);
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(at<W>(sq, row0 + r, c))
+                 : "memory");
+    if (first + r < wh.len) *reinterpret_cast<uint4*>(out + (long)r * p.o_stride + c * 8) = x;
   }
 }
 
 template <class T, int D>
 static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
-  constexpr int SMEM = 5 * 64 * 2 * D * 2;
+  constexpr int SMEM = 3 * 64 * 2 * D * 2;
   static std::mutex mu;
   static uint64_t attr_set = 0;  // per-device bit: the attribute is a per-device setting
   int dev = 0;
@@ -251,7 +317,7 @@ static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
     std::lock_guard<std::mutex> lk(mu);
     if (dev >= 64 || !(attr_set >> dev & 1)) {
       const cudaError_t e =
-          cudaFuncSetAttribute(diff_mma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+          cudaFuncSetAttribute(diff_short_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
       if (e != cudaSuccess) return e;
       if (dev < 64) attr_set |= 1ull << dev;
     }
@@ -259,7 +325,7 @@ static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg =
       pdl_config(dim3(block_count(p.T, p.nseq, BQ), p.heads), dim3(WARPS * 32), SMEM, s, attr);
-  return cudaLaunchKernelEx(&cfg, diff_mma_kernel<T, D>, p);
+  return cudaLaunchKernelEx(&cfg, diff_short_kernel<T, D>, p);
 }
 
 }  // namespace dif

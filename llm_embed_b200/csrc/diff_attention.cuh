@@ -23,16 +23,23 @@ struct Where {
 __device__ __forceinline__ bool find_block(const DiffParams& p, const int32_t* offsets, int tile, int bq, Where& w) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = p.nseq;  // the answer is in [lo, hi)
-  while (hi - lo > 1) {
+  int t0 = 0, t1 = 0;
+  while (true) {
     const int step = (hi - lo + 31) / 32;
     const int i = lo + lane * step;
-    const bool le = i < hi && (long)offsets[i] / bq + i <= tile;
+    const int at = i <= p.nseq ? offsets[i] : 0;
+    const bool le = i < hi && (long)at / bq + i <= tile;
     const int n = __popc(__ballot_sync(0xffffffffu, le));
     if (n == 0) return false;
     lo += (n - 1) * step;
     hi = min(hi, lo + step);
+    if (hi - lo <= 1) {  // its offsets: with steps of one, lanes n - 1 and n have them
+      t0 = __shfl_sync(0xffffffffu, at, n - 1);
+      t1 = __shfl_sync(0xffffffffu, at, n & 31);
+      if (step > 1 || n > 31) t1 = offsets[lo + 1];
+      break;
+    }
   }
-  const int t0 = offsets[lo], t1 = offsets[lo + 1];
   if (t0 < 0 || t1 < t0 || t1 > p.T) {
     if (lane == 0) report(p.status, DE_BOUNDS, 80, lo);
     return false;
