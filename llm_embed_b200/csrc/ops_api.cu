@@ -30,6 +30,10 @@ int le_fail(int code, const char* fmt, ...);
     if (r_ != LE_OK) return r_; \
   } while (0)
 
+// The Python binding packs these by field (llm_embed_b200/ops.py).
+static_assert(sizeof(le_f8gemm_args) == 72 && sizeof(le_qk_norm_args) == 112 && sizeof(le_diffattn_args) == 88,
+              "argument structures");
+
 namespace {
 
 // Makes `dev` current and the caller's device current again at the end.
@@ -63,32 +67,38 @@ struct Buf {
   }
 };
 
-// What every operator's handle has: its device, its own stream, the status
-// word that its kernels report to.
+// What every operator's handle has: its device, its own stream, and one
+// allocation with the status word that its kernels report to and its arrays
+// behind (256-byte steps).
 struct OpBase {
   int dev = 0;
   cudaStream_t stream = nullptr;
-  Buf status;
-  int open(int d) {
+  Buf mem;
+  static size_t step(size_t n) { return (n + 255) / 256 * 256; }
+  int open(int d, size_t bytes) {
     dev = d;
     CK(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking));
-    TRY(status.alloc(sizeof(DevStatus)));
-    CK(cudaMemset(status.p, 0, sizeof(DevStatus)));
+    TRY(mem.alloc(256 + bytes));
+    CK(cudaMemsetAsync(mem.p, 0, sizeof(DevStatus), cudaStreamLegacy));
     return LE_OK;
+  }
+  template <class T>
+  T* at(size_t offset) const {
+    return reinterpret_cast<T*>(mem.as<uint8_t>() + 256 + offset);
   }
   ~OpBase() {
     if (stream) cudaStreamDestroy(stream);
   }
   cudaStream_t pick(void* s) const { return s ? static_cast<cudaStream_t>(s) : stream; }
-  DevStatus* st() const { return status.as<DevStatus>(); }
+  DevStatus* st() const { return mem.as<DevStatus>(); }
   int sync() {
     DeviceGuard g(dev);
     CK(g.err);
     CK(cudaDeviceSynchronize());
     DevStatus h{};
-    CK(cudaMemcpy(&h, status.p, sizeof h, cudaMemcpyDeviceToHost));
+    CK(cudaMemcpy(&h, mem.p, sizeof h, cudaMemcpyDeviceToHost));
     if (h.code == DE_OK) return LE_OK;
-    CK(cudaMemset(status.p, 0, sizeof h));
+    CK(cudaMemset(mem.p, 0, sizeof h));
     return le_fail(LE_EDEVICE, "kernel failure code %d at site %d (info %d)", h.code, h.where, h.info);
   }
 };
@@ -136,18 +146,24 @@ struct Owner {
 }  // namespace
 
 struct le_f8weight : OpBase {
-  Buf w, ws;
   int N = 0, K = 0;
+  size_t w_bytes() const { return (size_t)N * K; }
+  size_t ws_bytes() const { return (size_t)(blocks128(N) * blocks128(K)) * 4; }
+  uint8_t* w() const { return at<uint8_t>(0); }
+  float* ws() const { return at<float>(step(w_bytes())); }
 };
 struct le_rope : OpBase {
-  Buf cos, sin;
   int max_pos = 0, rot = 0, half_split = 0;
+  size_t table_bytes() const { return (size_t)max_pos * (rot / 2) * 4; }
+  float* cos() const { return at<float>(0); }
+  float* sin() const { return at<float>(step(table_bytes())); }
 };
 struct le_diffattn : OpBase {
-  Buf lambda, norm_w;
   int heads = 0, kv_heads = 0, d = 0;
   float out_scale = 1.f, eps = 0.f;
   bool norm = false;
+  float* lambda() const { return at<float>(0); }
+  float* norm_w() const { return at<float>(step((size_t)heads * 4)); }
 };
 
 extern "C" {
@@ -180,12 +196,9 @@ static int f8weight_open(int dev, const void* src, int N, int K, Owner<le_f8weig
 }
 
 static int f8weight_alloc(le_f8weight* w, int dev, int N, int K) {
-  TRY(w->open(dev));
   w->N = N;
   w->K = K;
-  TRY(w->w.alloc((size_t)N * K));
-  TRY(w->ws.alloc((size_t)(blocks128(N) * blocks128(K)) * 4));
-  return LE_OK;
+  return w->open(dev, OpBase::step(w->w_bytes()) + w->ws_bytes());
 }
 
 int le_f8weight_create(int dev, const uint8_t* wq, const float* scales, int N, int K, le_f8weight** out) {
@@ -197,8 +210,8 @@ int le_f8weight_create(int dev, const uint8_t* wq, const float* scales, int N, i
   DeviceGuard g(dev);
   CK(g.err);
   TRY(f8weight_alloc(o.h, dev, N, K));
-  CK(cudaMemcpy(o.h->w.p, wq, (size_t)N * K, cudaMemcpyDefault));
-  CK(cudaMemcpy(o.h->ws.p, scales, (size_t)(blocks128(N) * blocks128(K)) * 4, cudaMemcpyDefault));
+  CK(cudaMemcpy(o.h->w(), wq, o.h->w_bytes(), cudaMemcpyDefault));
+  CK(cudaMemcpy(o.h->ws(), scales, o.h->ws_bytes(), cudaMemcpyDefault));
   CK(cudaStreamSynchronize(cudaStreamLegacy));
   *out = o.release();
   return LE_OK;
@@ -215,7 +228,7 @@ int le_f8weight_quantize(int dev, const float* w, int N, int K, le_f8weight** ou
   Buf src;
   TRY(src.alloc((size_t)N * K * 4));
   CK(cudaMemcpy(src.p, w, (size_t)N * K * 4, cudaMemcpyDefault));
-  CK(launch_f8_quantize_weight(src.as<float>(), N, K, o.h->w.as<uint8_t>(), o.h->ws.as<float>(), cudaStreamLegacy));
+  CK(launch_f8_quantize_weight(src.as<float>(), N, K, o.h->w(), o.h->ws(), cudaStreamLegacy));
   CK(cudaStreamSynchronize(cudaStreamLegacy));
   *out = o.release();
   return LE_OK;
@@ -225,8 +238,8 @@ int le_f8weight_read(le_f8weight* w, uint8_t* wq, float* scales) {
   if (!w) return le_fail(LE_EINVAL, "null argument");
   DeviceGuard g(w->dev);
   CK(g.err);
-  if (wq) CK(cudaMemcpy(wq, w->w.p, (size_t)w->N * w->K, cudaMemcpyDeviceToHost));
-  if (scales) CK(cudaMemcpy(scales, w->ws.p, (size_t)(blocks128(w->N) * blocks128(w->K)) * 4, cudaMemcpyDeviceToHost));
+  if (wq) CK(cudaMemcpy(wq, w->w(), w->w_bytes(), cudaMemcpyDeviceToHost));
+  if (scales) CK(cudaMemcpy(scales, w->ws(), w->ws_bytes(), cudaMemcpyDeviceToHost));
   return LE_OK;
 }
 
@@ -267,8 +280,8 @@ int le_f8gemm_device(le_f8weight* w, const le_f8gemm_args* a, void* stream) {
   const cudaStream_t s = w->pick(stream);
   p.x = a->x;
   p.xs = a->x_scales;
-  p.w = w->w.as<uint8_t>();
-  p.ws = w->ws.as<float>();
+  p.w = w->w();
+  p.ws = w->ws();
   p.y = a->y;
   int xt = a->x_type;
   // Up to F8_FUSED_MAX_M rows are quantised by the product's own kernel; more
@@ -305,15 +318,12 @@ int le_rope_create(int dev, int max_pos, int rot_dim, double base, int pairing, 
   if (!o.h) return le_fail(LE_ENOMEM, "out of host memory");
   DeviceGuard g(dev);
   CK(g.err);
-  TRY(o.h->open(dev));
   o.h->max_pos = max_pos;
   o.h->rot = rot_dim;
   o.h->half_split = pairing == LE_ROPE_HALF;
-  const size_t n = (size_t)max_pos * (rot_dim / 2) * 4;
-  TRY(o.h->cos.alloc(n));
-  TRY(o.h->sin.alloc(n));
-  CK(launch_rope_table(max_pos, rot_dim, base, o.h->cos.as<float>(), o.h->sin.as<float>(), o.h->stream));
-  CK(cudaStreamSynchronize(o.h->stream));
+  TRY(o.h->open(dev, OpBase::step(o.h->table_bytes()) + o.h->table_bytes()));
+  CK(launch_rope_table(max_pos, rot_dim, base, o.h->cos(), o.h->sin(), cudaStreamLegacy));
+  CK(cudaStreamSynchronize(cudaStreamLegacy));
   *out = o.release();
   return LE_OK;
 }
@@ -356,8 +366,8 @@ int le_qk_norm_device(le_rope* r, const le_qk_norm_args* a, void* stream) {
   p.max_pos = r->max_pos;
   p.q_weight = a->q_weight;
   p.k_weight = a->k_weight;
-  p.cos = r->cos.as<float>();
-  p.sin = r->sin.as<float>();
+  p.cos = r->cos();
+  p.sin = r->sin();
   p.positions = r->rot ? a->positions : nullptr;
   p.eps = a->eps;
   p.status = r->st();
@@ -387,14 +397,13 @@ int le_diffattn_create(int dev, int heads, int kv_heads, int head_dim, const flo
   if (!o.h) return le_fail(LE_ENOMEM, "out of host memory");
   DeviceGuard g(dev);
   CK(g.err);
-  TRY(o.h->open(dev));
   o.h->heads = heads;
   o.h->kv_heads = kv_heads;
   o.h->d = head_dim;
   o.h->out_scale = 1.f - lambda_init;
   o.h->eps = eps;
   o.h->norm = norm_weight != nullptr;
-  TRY(o.h->lambda.alloc((size_t)heads * 4));
+  TRY(o.h->open(dev, OpBase::step((size_t)heads * 4) + (size_t)2 * head_dim * 4));
   std::unique_ptr<float[]> lam(new (std::nothrow) float[heads]);
   if (!lam) return le_fail(LE_ENOMEM, "out of host memory");
   for (int i = 0; i < heads; i++) {
@@ -406,11 +415,9 @@ int le_diffattn_create(int dev, int heads, int kv_heads, int head_dim, const flo
     }
     lam[i] = (float)(std::exp(a) - std::exp(b) + (double)lambda_init);
   }
-  CK(cudaMemcpy(o.h->lambda.p, lam.get(), (size_t)heads * 4, cudaMemcpyHostToDevice));
-  if (norm_weight) {
-    TRY(o.h->norm_w.alloc((size_t)2 * head_dim * 4));
-    CK(cudaMemcpy(o.h->norm_w.p, norm_weight, (size_t)2 * head_dim * 4, cudaMemcpyHostToDevice));
-  }
+  CK(cudaMemcpy(o.h->lambda(), lam.get(), (size_t)heads * 4, cudaMemcpyHostToDevice));
+  if (norm_weight) CK(cudaMemcpy(o.h->norm_w(), norm_weight, (size_t)2 * head_dim * 4, cudaMemcpyHostToDevice));
+  CK(cudaStreamSynchronize(cudaStreamLegacy));
   *out = o.release();
   return LE_OK;
 }
@@ -443,21 +450,15 @@ int le_diffattn_device(le_diffattn* h, const le_diffattn_args* a, void* stream) 
   p.T = a->n_tokens;
   p.heads = h->heads;
   p.group = h->heads / h->kv_heads;
-  p.lambda = h->lambda.as<float>();
-  p.norm_w = h->norm ? h->norm_w.as<float>() : nullptr;
+  p.lambda = h->lambda();
+  p.norm_w = h->norm ? h->norm_w() : nullptr;
   p.out_scale = h->out_scale;
   p.eps = h->eps;
   p.status = h->st();
   DeviceGuard g(h->dev);
   CK(g.err);
   const cudaStream_t s = h->pick(stream);
-  const int path = getenv("LE_DIFF") ? atoi(getenv("LE_DIFF")) : 1;
-  p.min_len = 0;
-  p.max_len = 0x7fffffff;
-  if (path == 1)
-    CK(launch_diff_attention_tc(a->type, h->d, p, s));
-  else
-    CK(launch_diff_attention(a->type, h->d, p, s));
+  CK(launch_diff_attention(a->type, h->d, p, a->max_len, s));
   return LE_OK;
 }
 

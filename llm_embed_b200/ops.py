@@ -13,6 +13,7 @@ framework whose current stream has the handle 0 means it).  Element types are
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 
 import numpy as np
@@ -25,26 +26,11 @@ TYPES = {"f32": 0, "f16": 1, "bf16": 2, "e4m3": 3}
 PAIRINGS = {"interleaved": 0, "half": 1}
 
 
-class F8GemmArgs(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("x_scales", C.c_void_p), ("y", C.c_void_p), ("work", C.c_void_p),
-                ("work_bytes", C.c_int64), ("ldx", C.c_int64), ("ldy", C.c_int64), ("M", C.c_int32),
-                ("x_type", C.c_int32), ("y_type", C.c_int32)]
-
-
-class QkNormArgs(C.Structure):
-    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
-                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("positions", C.c_void_p),
-                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("q_out_stride", C.c_int64),
-                ("k_out_stride", C.c_int64), ("type", C.c_int32), ("n_tokens", C.c_int32), ("q_heads", C.c_int32),
-                ("k_heads", C.c_int32), ("head_dim", C.c_int32), ("eps", C.c_float)]
-
-
-class DiffAttnArgs(C.Structure):
-    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
-                ("offsets", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
-                ("out_stride", C.c_int64), ("type", C.c_int32), ("nseq", C.c_int32), ("n_tokens", C.c_int32),
-                ("max_len", C.c_int32)]
-
+# The argument structures of include/llmembed.h, field by field (packing one
+# takes a fraction of the time that building a ctypes.Structure does).
+_F8GEMM_ARGS = struct.Struct("@PPPPqqqiii4x").pack
+_QK_NORM_ARGS = struct.Struct("@PPPPPPPqqqqiiiiif").pack
+_DIFFATTN_ARGS = struct.Struct("@PPPPPqqqqiiii").pack
 
 _lib = None
 _lib_lock = threading.Lock()
@@ -64,11 +50,11 @@ def lib() -> C.CDLL:
                 L.le_f8weight_quantize.argtypes = [i, vp, i, i, out]
                 L.le_f8weight_read.argtypes = [vp, vp, vp]
                 L.le_f8gemm_workspace.argtypes = [vp, i, i, C.POINTER(i64)]
-                L.le_f8gemm_device.argtypes = [vp, C.POINTER(F8GemmArgs), vp]
+                L.le_f8gemm_device.argtypes = [vp, vp, vp]
                 L.le_rope_create.argtypes = [i, i, i, C.c_double, i, out]
-                L.le_qk_norm_device.argtypes = [vp, C.POINTER(QkNormArgs), vp]
+                L.le_qk_norm_device.argtypes = [vp, vp, vp]
                 L.le_diffattn_create.argtypes = [i, i, i, i, vp, i, C.c_float, vp, C.c_float, out]
-                L.le_diffattn_device.argtypes = [vp, C.POINTER(DiffAttnArgs), vp]
+                L.le_diffattn_device.argtypes = [vp, vp, vp]
                 for name in ("f8weight", "rope", "diffattn"):
                     getattr(L, f"le_{name}_sync").argtypes = [vp]
                     getattr(L, f"le_{name}_free").argtypes = [vp]
@@ -81,6 +67,17 @@ def _id(table: dict, name: str, what: str) -> int:
         return table[name]
     except (KeyError, TypeError):
         raise LlmEmbedError(LE_EINVAL, f"{what} {name!r} is none of {', '.join(table)}") from None
+
+
+def _run(fn, h, pack, stream: int, *args) -> None:
+    """fn(handle, packed arguments, stream), its code checked."""
+    try:
+        packed = pack(*args)
+    except (struct.error, TypeError) as e:
+        raise LlmEmbedError(LE_EINVAL, f"argument out of range or of another type: {e}") from None
+    rc = fn(h, packed, stream or None)
+    if rc:
+        _check(rc)
 
 
 class _Handle:
@@ -108,8 +105,10 @@ class _Handle:
 def f8_quantize_device(d_x: int, x_type: str, M: int, K: int, d_q: int, d_scales: int, ldx: int = 0, dev: int = 0,
                        stream: int = LEGACY_STREAM) -> None:
     """x [M][K] -> e4m3 bytes [M][K] and scales [ceil(K/128)][M] (le_f8_quantize_device)."""
-    _check(lib().le_f8_quantize_device(dev, _id(TYPES, x_type, "type"), d_x, ldx, M, K, d_q, d_scales,
-                                       stream or None))
+    rc = (_lib or lib()).le_f8_quantize_device(dev, _id(TYPES, x_type, "type"), d_x, ldx, M, K, d_q, d_scales,
+                                               stream or None)
+    if rc:
+        _check(rc)
 
 
 class F8Weight(_Handle):
@@ -153,9 +152,8 @@ class F8Weight(_Handle):
                       ldy: int = 0, d_x_scales: int = 0, d_work: int = 0, work_bytes: int = 0,
                       stream: int = 0) -> None:
         """y [M][N] = x [M][K] . W^T; x is quantised in the call, or e4m3 with d_x_scales."""
-        a = F8GemmArgs(d_x, d_x_scales, d_y, d_work, work_bytes, ldx, ldy, M, _id(TYPES, x_type, "type"),
-                       _id(TYPES, y_type, "type"))
-        _check(lib().le_f8gemm_device(self._h, C.byref(a), stream or None))
+        _run((_lib or lib()).le_f8gemm_device, self._h, _F8GEMM_ARGS, stream, d_x, d_x_scales, d_y, d_work, work_bytes,
+             ldx, ldy, M, _id(TYPES, x_type, "type"), _id(TYPES, y_type, "type"))
 
 
 def _address(a, dtype, n: int):
@@ -181,9 +179,9 @@ class Rope(_Handle):
                        d_positions: int, d_q_out: int, d_k_out: int, q_stride: int = 0, k_stride: int = 0,
                        q_out_stride: int = 0, k_out_stride: int = 0, d_q_weight: int = 0, d_k_weight: int = 0,
                        eps: float = 1e-6, stream: int = 0) -> None:
-        a = QkNormArgs(d_q, d_k, d_q_out, d_k_out, d_q_weight, d_k_weight, d_positions, q_stride, k_stride,
-                       q_out_stride, k_out_stride, _id(TYPES, dtype, "type"), n_tokens, q_heads, k_heads, head_dim, eps)
-        _check(lib().le_qk_norm_device(self._h, C.byref(a), stream or None))
+        _run((_lib or lib()).le_qk_norm_device, self._h, _QK_NORM_ARGS, stream, d_q, d_k, d_q_out, d_k_out, d_q_weight,
+             d_k_weight, d_positions, q_stride, k_stride, q_out_stride, k_out_stride, _id(TYPES, dtype, "type"),
+             n_tokens, q_heads, k_heads, head_dim, eps)
 
 
 class DiffAttention(_Handle):
@@ -208,6 +206,5 @@ class DiffAttention(_Handle):
     def run_device(self, dtype: str, d_q: int, d_k: int, d_v: int, d_offsets: int, nseq: int, n_tokens: int,
                    max_len: int, d_out: int, q_stride: int = 0, k_stride: int = 0, v_stride: int = 0,
                    out_stride: int = 0, stream: int = 0) -> None:
-        a = DiffAttnArgs(d_q, d_k, d_v, d_out, d_offsets, q_stride, k_stride, v_stride, out_stride,
-                         _id(TYPES, dtype, "type"), nseq, n_tokens, max_len)
-        _check(lib().le_diffattn_device(self._h, C.byref(a), stream or None))
+        _run((_lib or lib()).le_diffattn_device, self._h, _DIFFATTN_ARGS, stream, d_q, d_k, d_v, d_out, d_offsets,
+             q_stride, k_stride, v_stride, out_stride, _id(TYPES, dtype, "type"), nseq, n_tokens, max_len)
