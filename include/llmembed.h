@@ -295,7 +295,7 @@ int le_diffattn_free(le_diffattn* h);
  * accumulated device time and launch count per kernel class.  `launches`
  * counts every kernel this library launched for the model (profiling on or
  * off).  Classes: 0 QKV GEMM, 1 attention-output GEMM, 2 FFN up/gate GEMM,
- * 3 FFN down GEMM, 4 attention, 5 LayerNorm, 6 embedding gather + LN,
+ * 3 FFN down GEMM, 4 attention (and the norm of its heads), 5 LayerNorm, 6 embedding gather + LN,
  * 7 positions + mean-pool, 8 the single-kernel forward of small calls
  * (<= 16 tokens; all layers in one launch). */
 #define LE_NCLASS 9

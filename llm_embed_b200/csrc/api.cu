@@ -19,6 +19,7 @@
 
 #include "../../include/llmembed.h"
 #include "common.cuh"
+#include "elem.cuh"
 #include "gemm.h"
 #include "kernels.h"
 
@@ -148,6 +149,11 @@ struct QMat {
 struct Layer {
   QMat qkv, out, upgate, down;
   DevBuf attn_w, attn_b, out_w, out_b;
+  // Optional: norms of the query and key heads [head_dim]; differential
+  // attention's lambda [heads / 2], norm [2 head_dim] and 1 - lambda_init.
+  DevBuf q_norm, k_norm, diff_lambda, diff_norm;
+  bool head_norm = false, diff = false;
+  float diff_scale = 1.f;
 };
 
 struct Workspace {
@@ -460,6 +466,51 @@ static int gemm(le_model* m, int cls, const QMat& W, const __half* A, int lda, c
     m->prof.end(s);         \
   } while (0)
 
+// A layer's attention parts that the reference lacks, on the packed QKV rows:
+// norm and rotation of the heads in place (qk_norm.cu), differential attention
+// over pairs of heads (diff_attention.cu).
+static cudaError_t launch_head_norm(const le_model* m, const Layer& L, __half* qkv, const int32_t* pos, int T,
+                                    cudaStream_t s) {
+  const int H = m->hp.hidden;
+  QkNormParams p{};
+  p.q = p.q_out = qkv;
+  p.k = p.k_out = qkv + H;
+  p.q_stride = p.k_stride = p.qo_stride = p.ko_stride = 3L * H;
+  p.q_heads = p.k_heads = m->hp.heads;
+  p.d = p.rot = m->head_dim;
+  p.max_pos = m->hp.context_length;
+  p.q_weight = L.q_norm.as<float>();
+  p.k_weight = L.k_norm.as<float>();
+  p.cos = m->rope_cos.as<float>();
+  p.sin = m->rope_sin.as<float>();
+  p.positions = pos;
+  p.eps = m->hp.ln_eps;
+  p.status = m->status.as<DevStatus>();
+  return launch_qk_norm(DT_F16, p, T, s);
+}
+static DiffParams diff_params(const le_model* m, const Layer& L, const __half* qkv, const int32_t* offsets, int nseq,
+                              int T, __half* att) {
+  const int H = m->hp.hidden;
+  DiffParams p{};
+  p.q = qkv;
+  p.k = qkv + H;
+  p.v = qkv + 2 * H;
+  p.out = att;
+  p.q_stride = p.k_stride = p.v_stride = 3L * H;
+  p.o_stride = H;
+  p.offsets = offsets;
+  p.nseq = nseq;
+  p.T = T;
+  p.heads = m->hp.heads / 2;
+  p.group = 1;
+  p.lambda = L.diff_lambda.as<float>();
+  p.norm_w = L.diff_norm.as<float>();
+  p.out_scale = L.diff_scale;
+  p.eps = m->hp.ln_eps;
+  p.status = m->status.as<DevStatus>();
+  return p;
+}
+
 // bert.go:216-285 (Forward) for packed sequences + pool.go (MeanPool,
 // L2Normalize) + embedder.go:66-68 (truncation), all enqueued on `s`.
 static int forward(le_model* m, const int32_t* d_ids, const int32_t* d_offsets, int nseq, int T, int max_len,
@@ -476,7 +527,9 @@ static int forward(le_model* m, const int32_t* d_ids, const int32_t* d_offsets, 
   unsigned long long* ln_part = w.ln_part.as<unsigned long long>();
   unsigned* ln_ctl = w.ln_ctl.as<unsigned>();
   const int ln_rows = gemm_ln_part_rows(w.cap_tokens);
-  if (T > 0 && T <= SMALL_MAX_TOKENS && (int)m->layers.size() <= SMALL_MAX_LAYERS) {
+  bool plain = true;  // every layer's attention is the reference's
+  for (const Layer& L : m->layers) plain = plain && !L.head_norm && !L.diff;
+  if (plain && T > 0 && T <= SMALL_MAX_TOKENS && (int)m->layers.size() <= SMALL_MAX_LAYERS) {
     // A few tokens: the whole encoder and the pool in one cooperative kernel.
     SmallParams sp{};
     sp.T = T;
@@ -546,14 +599,19 @@ static int forward(le_model* m, const int32_t* d_ids, const int32_t* d_offsets, 
       e.rope_cos = m->rope_cos.as<float>();
       e.rope_sin = m->rope_sin.as<float>();
       e.head_dim = m->head_dim;
-      e.rope_cols = 2 * H;
+      e.rope_cols = L.head_norm ? 0 : 2 * H;
       TRY(gemm(m, 0, L.qkv, hA, H, e, s));
-      if (att_tc)
+      if (L.head_norm) PLAUNCH(4, launch_head_norm(m, L, qkv, pos, T, s));
+      if (L.diff) {
+        const DiffParams dp = diff_params(m, L, qkv, d_offsets, nseq, T, att);
+        m->prof.launches += diff_attention_launches(dp, max_len) - 1;
+        PLAUNCH(4, launch_diff_attention(DT_F16, m->head_dim, dp, max_len, s));
+      } else if (att_tc)
         PLAUNCH(4, launch_attention_stc(qkv, w.att_units.p, w.cap_seqs, nseq, T, H, m->hp.heads, att,
                                         m->status.as<DevStatus>(), s));
       else
         PLAUNCH(4, launch_attention(qkv, d_offsets, nseq, max_len, H, m->hp.heads, m->head_dim, att, s));
-      if (max_len > ATTN_SHORT_MAX)
+      if (!L.diff && max_len > ATTN_SHORT_MAX)
         PLAUNCH(4, launch_attention_tc(qkv, d_offsets, nseq, T, max_len, ATTN_SHORT_MAX + 1, H, m->hp.heads, att,
                                        m->status.as<DevStatus>(), s));
       EpiParams r{};
@@ -824,6 +882,52 @@ static const le_tensor_desc* find(const le_tensor_desc* t, int nt, const std::st
   return nullptr;
 }
 
+// Optional tensors of a layer that the reference does not know: head norms and
+// differential attention.
+static int load_layer_extras(const le_model* m, Layer& L, int i, const le_tensor_desc* ts, int nt, cudaStream_t s) {
+  const std::string p = "blk." + std::to_string(i) + ".";
+  const int d = m->head_dim;
+  auto sized = [&](const le_tensor_desc* t, int64_t n) {
+    int64_t have = 1;
+    for (int k = 0; k < t->n_dims; k++) have *= t->dims[k];
+    return have == n ? LE_OK : fail(LE_EINVAL, "%s has %lld elements, expected %lld", t->name, (long long)have, (long long)n);
+  };
+  const le_tensor_desc *qn = find(ts, nt, p + "attn_q_norm.weight"), *kn = find(ts, nt, p + "attn_k_norm.weight");
+  if (!qn != !kn) return fail(LE_EINVAL, "%sattn_q_norm.weight and attn_k_norm.weight come together", p.c_str());
+  if (qn) {
+    TRY(sized(qn, d));
+    TRY(sized(kn, d));
+    TRY(upload_f32(L.q_norm, qn, d, s));
+    TRY(upload_f32(L.k_norm, kn, d, s));
+    L.head_norm = true;
+  }
+  const le_tensor_desc *dl = find(ts, nt, p + "attn_diff_lambda.weight"), *dn = find(ts, nt, p + "attn_diff_norm.weight");
+  if (!dl != !dn) return fail(LE_EINVAL, "%sattn_diff_lambda.weight and attn_diff_norm.weight come together", p.c_str());
+  if (dl) {
+    if (m->hp.heads % 2) return fail(LE_EINVAL, "differential attention needs an even number of heads (%d)", m->hp.heads);
+    TRY(sized(dl, 4 * d));
+    TRY(sized(dn, 2 * d));
+    if (dl->type != T_F32 || dl->n_bytes < 16 * d) return fail(LE_EINVAL, "tensor %s must be F32", dl->name);
+    TRY(upload_f32(L.diff_norm, dn, 2 * d, s));
+    // lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init of the layer's depth.
+    const double init = 0.8 - 0.6 * std::exp(-0.3 * i);
+    std::vector<float> l(4 * (size_t)d);
+    std::memcpy(l.data(), dl->data, l.size() * 4);
+    double a = 0, b = 0;
+    for (int k = 0; k < d; k++) {
+      a += (double)l[k] * l[d + k];
+      b += (double)l[2 * d + k] * l[3 * d + k];
+    }
+    const std::vector<float> lam(m->hp.heads / 2, (float)(std::exp(a) - std::exp(b) + init));
+    TRY(L.diff_lambda.ensure(lam.size() * 4));
+    CK(cudaMemcpyAsync(L.diff_lambda.p, lam.data(), lam.size() * 4, cudaMemcpyHostToDevice, s));
+    CK(cudaStreamSynchronize(s));
+    L.diff_scale = (float)(1.0 - init);
+    L.diff = true;
+  }
+  return LE_OK;
+}
+
 static int load_impl(int dev, const le_tensor_desc* ts, int nt, const le_hparams* hp, le_model** out,
                      double parse_ms = 0) {
   const double t_start = now_ms();
@@ -928,6 +1032,7 @@ static int load_impl(int dev, const le_tensor_desc* ts, int nt, const le_hparams
       if (!t) return fail(LE_EINVAL, "tensor \"%s%s\" not found", p.c_str(), nn[j]);
       TRY(upload_f32(*dst[j], t, H, s));
     }
+    TRY(load_layer_extras(m.get(), L, i, ts, nt, s));
   }
   // ops_simd.go:107-124 (NewRoPETable): freq = f32(1)/f32(pow(base, 2i/d)),
   // theta = freq * f32(pos), cos/sin in float64 rounded to float32.
@@ -1012,6 +1117,7 @@ int le_model_load_stats(const le_model* m, le_load_stats* out) {
   for (const Layer& L : m->layers) {
     for (const QMat* q : {&L.qkv, &L.out, &L.upgate, &L.down}) dev_bytes += q->buf.n + q->r16.n + q->w16.n;
     dev_bytes += L.attn_w.n + L.attn_b.n + L.out_w.n + L.out_b.n;
+    dev_bytes += L.q_norm.n + L.k_norm.n + L.diff_lambda.n + L.diff_norm.n;
   }
   out->weight_bytes = (int64_t)dev_bytes;
   return LE_OK;

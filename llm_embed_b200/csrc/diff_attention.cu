@@ -335,20 +335,28 @@ static cudaError_t launch_short(int dt, int d, const DiffParams& p, cudaStream_t
   return d == 64 ? dif::launch<__nv_bfloat16, 64>(p, s) : dif::launch<__nv_bfloat16, 32>(p, s);
 }
 
+// Texts of at most 64 tokens: this file's kernel (256 of 16 tokens, 6 heads of
+// 64: 13 us, tcgen05 tiles 46; 256 of 64: 38 and 47).  Else the tiles (64 of 128:
+// 49 and 21 us; 256 of 16 to 128: 57 us, and 68 with the short ones taken out),
+// with the short ones taken out where nearly all are.
+enum Plan { PLAN_SHORT, PLAN_TILES, PLAN_BOTH };
+static Plan plan_of(const DiffParams& p, int max_len) {
+  if (max_len > 0 && max_len <= dif::BKEY) return PLAN_SHORT;
+  return (long)p.T < 40L * p.nseq ? PLAN_BOTH : PLAN_TILES;
+}
+int diff_attention_launches(const DiffParams& p, int max_len) {
+  return p.nseq == 0 || p.T == 0 ? 0 : plan_of(p, max_len) == PLAN_BOTH ? 2 : 1;
+}
+
 cudaError_t launch_diff_attention(int dt, int d, const DiffParams& params, int max_len, cudaStream_t s) {
   if (params.nseq == 0 || params.T == 0) return cudaSuccess;
+  const Plan plan = plan_of(params, max_len);
   DiffParams p = params;
   p.min_len = 0;
-  p.max_len = 0x7fffffff;
-  // Texts of at most 64 tokens: this file's kernel (256 of 16 tokens, 6 heads
-  // of 64: 13 us, tcgen05 tiles 46; 256 of 64: 38 and 47).
-  if (max_len > 0 && max_len <= dif::BKEY) return launch_short(dt, d, p, s);
-  // Else the tiles (64 of 128: 49 and 21 us; 256 of 16 to 128: 57 us, and 68 with
-  // the short ones taken out), unless nearly all sequences are short.
-  if ((long)p.T < 40L * p.nseq) {
-    p.max_len = dif::BKEY;
+  p.max_len = plan == PLAN_BOTH ? dif::BKEY : 0x7fffffff;
+  if (plan != PLAN_TILES) {
     const cudaError_t e = launch_short(dt, d, p, s);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || plan == PLAN_SHORT) return e;
     p.min_len = dif::BKEY + 1;
   }
   return launch_diff_attention_tc(dt, d, p, s);

@@ -175,6 +175,7 @@ struct DiffParams {
 // max_len: the longest sequence if known, else 0; it chooses the kernels, which
 // are right for any length.
 cudaError_t launch_diff_attention(int dt, int d, const DiffParams& p, int max_len, cudaStream_t s);
+int diff_attention_launches(const DiffParams& p, int max_len);  // kernels of such a call
 // diff_attention_tc.cu: tcgen05 tiles of 128 queries and 64 keys, sequences of
 // at least min_len tokens; the other is for at most max_len (diff_attention.cu).
 cudaError_t launch_diff_attention_tc(int dt, int d, const DiffParams& p, cudaStream_t s);

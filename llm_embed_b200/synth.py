@@ -187,6 +187,10 @@ class ModelSpec:
     seed: int = 0
     std: float = 0.02
     tokens: bool = True  # write tokenizer.ggml.tokens (tokenizer.go:24)
+    # tensors of newer encoder layers: norms of the query and key heads,
+    # differential attention's learned weights and its norm
+    qk_norm: bool = False
+    diff_attn: bool = False
 
 
 CONFIG_SPECS = {
@@ -215,12 +219,20 @@ def _tensor_list(spec: ModelSpec):
             if w == "attn_output":
                 t.append((p + "attn_output_norm.weight", [H], GGML_F32))
                 t.append((p + "attn_output_norm.bias", [H], GGML_F32))
+                d = H // spec.heads
+                if spec.qk_norm:
+                    t += [(p + "attn_q_norm.weight", [d], GGML_F32), (p + "attn_k_norm.weight", [d], GGML_F32)]
+                if spec.diff_attn:
+                    t += [(p + "attn_diff_lambda.weight", [d, 4], GGML_F32), (p + "attn_diff_norm.weight", [2 * d], GGML_F32)]
         t.append((p + "layer_output_norm.weight", [H], GGML_F32))
         t.append((p + "layer_output_norm.bias", [H], GGML_F32))
     return t
 
 
 def _tensor_data(spec: ModelSpec, idx: int, name: str, dims, gtype: int) -> bytes:
+    if any(s in name for s in ("attn_q_norm", "attn_k_norm", "attn_diff_")):
+        w = np.random.default_rng([spec.seed, idx]).standard_normal(int(np.prod(dims)), dtype=np.float32)
+        return (0.1 * w if "lambda" in name else 1 + 0.2 * w).astype(np.float32).tobytes()
     if name.endswith("norm.weight"):
         return np.ones(dims[0], np.float32).tobytes()
     if name.endswith("norm.bias"):
@@ -301,6 +313,7 @@ def cached_model(name_or_spec, directory: str | None = None) -> str:
     tag = "_".join(str(x) for x in (spec.layers, spec.hidden, spec.heads, spec.ffn, spec.vocab, spec.context,
                                       spec.embd_type, *spec.weight_types, spec.seed,
                                       int(spec.tokens) * VOCAB_VERSION))
+    tag += "_qkn" * spec.qk_norm + "_diff" * spec.diff_attn
     path = os.path.join(directory, f"nomic_{tag}.gguf")
     if not os.path.exists(path):
         write_model(path, spec)
