@@ -176,7 +176,6 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
   if constexpr (CG == 2) cluster_sync();  // both CTAs' barriers are initialised before any remote arrive
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();  // the quantised activations are the previous kernel's
   pdl_trigger();
   // The widest tile's epilogue holds 128 sums a thread: of the 384 x 168
   // registers at launch the first warpgroup keeps 40 each, the two of the
@@ -188,27 +187,33 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     if (lane == 0) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_a)) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_b)) : "memory");
+      auto load = [&](const CUtensorMap* map, uint32_t dst, int kb, int row, int s) {
+        if constexpr (CG == 2)
+          tma_load_2d_pair(dst, map, kb * BK, row, map_to_rank(full(s), 0));
+        else
+          tma_load_2d(dst, map, kb * BK, row, full(s));
+      };
+      auto load_weight = [&](int tile, int kb, int s) {
+        if (leader) mbar_expect_tx(full(s), CG * (C::A_BYTES + C::B_BYTES));
+        load(&tmap_b, sbase + C::OFF_B + s * C::B_BYTES, kb, tile % n_tiles * BN + (int)rank * C::B_ROWS, s);
+      };
+      // The weight is no other kernel's result: the first stages' part of it is
+      // on its way before the previous kernel (the quantiser) has ended.
+      const int early = min(S, KB);
+      for (int kb = 0; kb < early; kb++) load_weight(first, kb, kb);
+      pdl_wait();
       uint32_t it = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += step) {
-        const int mt = tile / n_tiles, nt = tile % n_tiles;
-        const int row = (mt * CG + (int)rank) * BM, col = nt * BN + (int)rank * C::B_ROWS;
+        const int row = (tile / n_tiles * CG + (int)rank) * BM;
         for (int kb = 0; kb < KB; kb++, it++) {
           const int s = it % S;
           if (!mbar_wait(empty(s), ((it / S) & 1) ^ 1, abort_flag, status, 50)) {
             ok = false;
             break;
           }
-          if (leader) mbar_expect_tx(full(s), CG * (C::A_BYTES + C::B_BYTES));
-          const uint32_t a = sbase + C::OFF_A + s * C::A_BYTES, b = sbase + C::OFF_B + s * C::B_BYTES;
-          if constexpr (CG == 2) {
-            const uint32_t bar = map_to_rank(full(s), 0);
-            tma_load_2d_pair(a, &tmap_a, kb * BK, row, bar);
-            tma_load_2d_pair(b, &tmap_b, kb * BK, col, bar);
-          } else {
-            tma_load_2d(a, &tmap_a, kb * BK, row, full(s));
-            tma_load_2d(b, &tmap_b, kb * BK, col, full(s));
-          }
+          if (it >= (uint32_t)early) load_weight(tile, kb, s);
+          load(&tmap_a, sbase + C::OFF_A + s * C::A_BYTES, kb, row, s);
         }
       }
     }
@@ -268,6 +273,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         w1 = __ldg(ws + 1);
       }
     };
+    pdl_wait();  // the scales and y's memory are the previous kernels'
     first_scales(first);
     for (int tile = first; tile < total && ok; tile += step) {
       const int mt = tile / n_tiles, nt = tile % n_tiles;
