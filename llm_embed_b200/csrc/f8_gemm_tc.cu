@@ -107,20 +107,46 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
                  "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
-// Plain stores of 32 rows x 32 columns staged in the warp's shared memory:
-// consecutive lanes write consecutive columns of a row.
+// Plain stores of 32 rows x 128 bytes (words[32] of a lane: its row), turned in
+// the warp's shared memory so that consecutive lanes write consecutive words of
+// a row (word j of row i lies at j ^ i: distinct banks both ways).  `even`:
+// rows begin on 4-byte boundaries; else a word of two columns goes out in
+// halves.
 template <class Y>
-__device__ __forceinline__ void store_plain(float* stg, const float* v, Y* y, long ldy, int row0, int col0, int M,
-                                            int N) {
+__device__ __forceinline__ void store_plain(uint32_t* stg, const uint32_t* words, Y* y, long ldy, int row0, int col0,
+                                            int M, int N, bool even) {
   const int lane = threadIdx.x & 31;
+  __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 32; j++) stg[lane * 33 + j] = v[j];
+  for (int j = 0; j < 32; j++) stg[lane * 32 + (j ^ lane)] = words[j];
   __syncwarp();
-  if (col0 + lane < N) {
-    const int n = min(32, M - row0);
-    for (int i = 0; i < n; i++) y[(long)(row0 + i) * ldy + col0 + lane] = from_f32<Y>(stg[i * 33 + lane]);
+  constexpr int PER = 4 / sizeof(Y);  // columns of a word
+  const int col = col0 + lane * PER, n = min(32, M - row0);
+  Y* out = y + (long)row0 * ldy + col;
+  if (n == 32 && col0 + 32 * PER <= N) {  // a whole block: nothing to decide in the loops
+    if (PER == 1 || even) {
+#pragma unroll
+      for (int i = 0; i < 32; i++, out += ldy) *reinterpret_cast<uint32_t*>(out) = stg[i * 32 + (lane ^ i)];
+    } else {
+#pragma unroll 8
+      for (int i = 0; i < 32; i++, out += ldy) {
+        const uint32_t w = stg[i * 32 + (lane ^ i)];
+        reinterpret_cast<uint16_t*>(out)[0] = (uint16_t)w;
+        reinterpret_cast<uint16_t*>(out)[1] = (uint16_t)(w >> 16);
+      }
+    }
+    return;
   }
-  __syncwarp();
+#pragma unroll 4
+  for (int i = 0; i < n; i++, out += ldy) {
+    const uint32_t w = stg[i * 32 + (lane ^ i)];
+    if constexpr (PER == 1) {
+      if (col < N) *reinterpret_cast<uint32_t*>(out) = w;
+    } else {
+      if (col < N) reinterpret_cast<uint16_t*>(out)[0] = (uint16_t)w;
+      if (col + 1 < N) reinterpret_cast<uint16_t*>(out)[1] = (uint16_t)(w >> 16);
+    }
+  }
 }
 
 template <class C, class Y>
@@ -253,7 +279,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     const int quarter = warp & 3, ew = warp - EPI_WARP0;
     const int c0 = (ew >> 2) * COLS;  // this warp's columns of the tile
     const uint32_t stage = sbase + C::OFF_STAGE + ew * 2 * 4096;
-    float* stg = reinterpret_cast<float*>(smem + C::OFF_STAGE + ew * 2 * 4096);
+    uint32_t* stg = reinterpret_cast<uint32_t*>(smem + C::OFF_STAGE + ew * 2 * 4096);
+    const bool even = p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
     int buf = 0;
     uint32_t it = 0;
     bool ok = true;
@@ -325,33 +352,26 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       if (!ok) break;
       first_scales(tile + step);  // on their way during the stores
       if (row0 >= p.M) continue;  // warp-uniform
-      if (use_tma) {
-        constexpr int PER = 128 / sizeof(Y);  // columns of a 128-byte block
+      constexpr int PER = 128 / sizeof(Y);  // columns of a 128-byte block
 #pragma unroll
-        for (int c = 0; c < COLS; c += PER) {
-          if (n0 + c >= p.N) break;
-          uint32_t words[32];
+      for (int c = 0; c < COLS; c += PER) {
+        if (n0 + c >= p.N) break;
+        uint32_t words[32];
 #pragma unroll
-          for (int i = 0; i < PER / 2; i++) {
-            float lo, hi;
-            f2_unpack(acc[c / 2 + i], lo, hi);
-            if constexpr (sizeof(Y) == 4) {
-              words[2 * i] = __float_as_uint(lo);
-              words[2 * i + 1] = __float_as_uint(hi);
-            } else {
-              words[i] = pack2<Y>(lo, hi);
-            }
+        for (int i = 0; i < PER / 2; i++) {
+          float lo, hi;
+          f2_unpack(acc[c / 2 + i], lo, hi);
+          if constexpr (sizeof(Y) == 4) {
+            words[2 * i] = __float_as_uint(lo);
+            words[2 * i + 1] = __float_as_uint(hi);
+          } else {
+            words[i] = pack2<Y>(lo, hi);
           }
+        }
+        if (use_tma)
           emit_block(&tmap_y, stage, buf, words, n0 + c, row0);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 16; i++) f2_unpack(acc[c / 2 + i], v[2 * i], v[2 * i + 1]);
-          store_plain<Y>(stg, v, static_cast<Y*>(p.y), p.ldy, row0, n0 + c, p.M, p.N);
-        }
+        else
+          store_plain<Y>(stg, words, static_cast<Y*>(p.y), p.ldy, row0, n0 + c, p.M, p.N, even);
       }
     }
     if (use_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
