@@ -59,20 +59,25 @@ __device__ __forceinline__ uint32_t at(uint32_t base, int row, int chunk) {
   return base + row * (W * 2) + ((chunk ^ (row & 7)) << 4);
 }
 
-// 64 rows of a tile: row r is token r % per of head r / per, from src + token *
-// ld + head * W; tokens from `n` on and heads from `heads` on are zero.  GROUP
-// query heads share a head of src.
+// 64 rows of a tile, 2^lg to a head: row r is token r % 2^lg of head r / 2^lg,
+// from src + token * ld + head * W; tokens from `n` on and heads from `heads` on
+// are zero.  `group` query heads share a head of src.  A thread keeps its chunk
+// and goes down the rows in steps whose token and head are the same for the
+// whole CTA.
 template <int W, class T>
-__device__ __forceinline__ void load_tile(uint32_t base, const T* src, long ld, int per, int n, int head0, int heads,
+__device__ __forceinline__ void load_tile(uint32_t base, const T* src, long ld, int lg, int n, int head0, int heads,
                                           int group) {
-  constexpr int CH = W / 8;
+  constexpr int CH = W / 8, STEP = WARPS * 32 / CH;  // 8 or 16 rows
+  const int r0 = threadIdx.x / CH, c = threadIdx.x % CH;
+  const T* mine = src + (long)r0 * ld + c * 8;
+  const uint32_t dst = at<W>(base, r0, c);
 #pragma unroll
-  for (int k = 0; k < 64 * CH / (WARPS * 32); k++) {
-    const int i = k * (WARPS * 32) + threadIdx.x, r = i / CH, c = i % CH;
-    const int token = r & (per - 1), head = head0 + r / per;
-    const bool in = token < n && head < heads;
-    const T* g = src + (long)(in ? token : 0) * ld + (long)((in ? head : head0) / group) * W + c * 8;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at<W>(base, r, c)), "l"(g), "r"(in ? 16 : 0));
+  for (int r = 0; r < 64; r += STEP) {
+    const int token = r & ((1 << lg) - 1), head = head0 + (r >> lg);
+    const int h = group == 1 ? head : head / group;
+    const bool in = token + r0 < n && head < heads;
+    const T* g = in ? mine + (long)token * ld + h * W : src;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * (W * 2)), "l"(g), "r"(in ? 16 : 0));
   }
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -145,125 +150,56 @@ __device__ __forceinline__ void add_block(Stat& st, float (&s)[8][4], float scal
   st.m[1] = m1;
 }
 
-// o += P V for the weights w1 a - w2 b of the first `left` keys from key0.
+// P = w1 a - w2 b as the second product's operand.
+template <class T>
+__device__ __forceinline__ void weights(uint32_t (&pa)[BKEY / 16][4], const float (&a)[8][4], const float (&b)[8][4],
+                                        const float (&w1)[2], const float (&w2)[2]) {
+#pragma unroll
+  for (int n = 0; n < 8; n++) {
+    pa[n / 2][2 * (n & 1)] = pack2<T>(fmaf(a[n][0], w1[0], -b[n][0] * w2[0]), fmaf(a[n][1], w1[0], -b[n][1] * w2[0]));
+    pa[n / 2][2 * (n & 1) + 1] = pack2<T>(fmaf(a[n][2], w1[1], -b[n][2] * w2[1]), fmaf(a[n][3], w1[1], -b[n][3] * w2[1]));
+  }
+}
+
+// o += P V for the first `left` keys from key0.
 template <class T, int W>
-__device__ __forceinline__ void values(float (&o)[W / 8][4], const float (&a)[8][4], const float (&b)[8][4],
-                                       const float (&w1)[2], const float (&w2)[2], uint32_t sv, int key0, int left) {
+__device__ __forceinline__ void values(float (&o)[W / 8][4], const uint32_t (&pa)[BKEY / 16][4], uint32_t sv, int key0,
+                                       int left) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int c = 0; c < BKEY / 16; c++)
     if (c * 16 < left) {
-      uint32_t pa[4];
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int n = 2 * c + h;
-        pa[2 * h] = pack2<T>(fmaf(a[n][0], w1[0], -b[n][0] * w2[0]), fmaf(a[n][1], w1[0], -b[n][1] * w2[0]));
-        pa[2 * h + 1] = pack2<T>(fmaf(a[n][2], w1[1], -b[n][2] * w2[1]), fmaf(a[n][3], w1[1], -b[n][3] * w2[1]));
-      }
 #pragma unroll
       for (int n = 0; n < W / 8; n += 2) {
         uint32_t f[4];
         ldsm4_t(f, at<W>(sv, key0 + c * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, n + (lane >> 4)));
-        mma16<T>(o[n], pa, f[0], f[1]);
-        mma16<T>(o[n + 1], pa, f[2], f[3]);
+        mma16<T>(o[n], pa[c], f[0], f[1]);
+        mma16<T>(o[n + 1], pa[c], f[2], f[3]);
       }
     }
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(WARPS * 32, 3) diff_short_kernel(DiffParams p) {
-  constexpr int W = 2 * D, TILE = 64 * W * 2;
-  pdl_wait();
-  pdl_trigger();
-  if (blockIdx.x == 0 && blockIdx.y == 0) check_offsets(p, WARPS * 32);
-  Where wh;
-  if (!find_block(p, p.offsets, blockIdx.x, BQ, wh) || wh.len < p.min_len || wh.len > p.max_len) return;
-  const int per = wh.len <= 16 ? 16 : wh.len <= 32 ? 32 : 64;  // rows of a head in the tiles
-  const int head0 = blockIdx.y * (64 / per);
-  if (head0 >= p.heads) return;
-  extern __shared__ __align__(128) uint8_t smem_diff[];
-  const uint32_t sq = (uint32_t)__cvta_generic_to_shared(smem_diff), sk = sq + TILE, sv = sk + TILE;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row0 = warp * 16, key0 = row0 & ~(per - 1);      // in the tiles
-  const int head = head0 + row0 / per, first = wh.q0 + (row0 & (per - 1));  // the warp's head and first token
-  const bool work = head < p.heads && first < wh.len;        // warp-uniform
-  const T* q = static_cast<const T*>(p.q) + (long)(wh.t0 + wh.q0) * p.q_stride;
-  const T* k = static_cast<const T*>(p.k) + (long)wh.t0 * p.k_stride;
-  const T* v = static_cast<const T*>(p.v) + (long)wh.t0 * p.v_stride;
-  const float scale = 1.4426950408889634f * rsqrtf((float)D);
-  const float lambda = work ? p.lambda[head] : 0.f;
-  float o[W / 8][4];
-#pragma unroll
-  for (int n = 0; n < W / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+// Where a warp's 16 rows lie: in the tiles, and which head and tokens they are.
+struct Rows {
+  int row0, key0, head, first;
+  bool work;  // any of them is the sequence's
+};
+__device__ __forceinline__ Rows rows_of(const DiffParams& p, const Where& wh, int lg, int head0) {
+  Rows r;
+  r.row0 = (threadIdx.x >> 5) * 16;
+  r.key0 = r.row0 >> lg << lg;
+  r.head = head0 + (r.row0 >> lg);
+  r.first = wh.q0 + r.row0 - r.key0;
+  r.work = r.head < p.heads && r.first < wh.len;
+  return r;
+}
 
-  load_tile<W>(sq, q, p.q_stride, per, wh.len - wh.q0, head0, p.heads, 1);
-  Stat st[2];
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    st[i].m[0] = st[i].m[1] = -INFINITY;
-    st[i].l[0] = st[i].l[1] = 0.f;
-  }
-  if (wh.len <= BKEY) {
-    load_tile<W>(sk, k, p.k_stride, per, wh.len, head0, p.heads, p.group);
-    commit_copies();
-    load_tile<W>(sv, v, p.v_stride, per, wh.len, head0, p.heads, p.group);
-    commit_copies();
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    __syncthreads();
-    float s[2][8][4];
-    if (work) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        scores<T, D>(s[i], sq, sk, i, row0, key0, wh.len);
-        add_block(st[i], s[i], scale);
-      }
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
-    if (!work) return;
-    const float w1[2] = {1.f / st[0].l[0], 1.f / st[0].l[1]};
-    const float w2[2] = {lambda / st[1].l[0], lambda / st[1].l[1]};
-    values<T, W>(o, s[0], s[1], w1, w2, sv, key0, wh.len);
-  } else {
-    for (int pass = 0; pass < 2; pass++) {
-      float w1[2], w2[2];
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        w1[r] = 1.f / st[0].l[r];
-        w2[r] = lambda / st[1].l[r];
-      }
-      for (int j = 0; j * BKEY < wh.len; j++) {
-        const int left = wh.len - j * BKEY;
-        load_tile<W>(sk, k + (long)j * BKEY * p.k_stride, p.k_stride, per, left, head0, p.heads, p.group);
-        if (pass == 1) load_tile<W>(sv, v + (long)j * BKEY * p.v_stride, p.v_stride, per, left, head0, p.heads, p.group);
-        commit_copies();
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();
-        if (work) {
-          float s[2][8][4];
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            scores<T, D>(s[i], sq, sk, i, row0, 0, left);
-            if (pass == 0) {
-              add_block(st[i], s[i], scale);
-            } else {
-#pragma unroll
-              for (int n = 0; n < 8; n++)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                  s[i][n][e] = ex2f(fmaf(s[i][n][e], scale, -st[i].m[e >> 1] * scale));
-            }
-          }
-          if (pass == 1) values<T, W>(o, s[0], s[1], w1, w2, sv, 0, left);
-        }
-        __syncthreads();
-      }
-    }
-    if (!work) return;
-  }
-
-  // Norm, then out through the warp's own rows of the query tile: whole
-  // 16-byte chunks of a row instead of pairs of elements.
+// Norm, then out through the warp's own rows of the query tile: whole 16-byte
+// chunks of a row instead of pairs of elements.
+template <class T, int W>
+__device__ __forceinline__ void finish(const DiffParams& p, const Where& wh, const Rows& rw, float (&o)[W / 8][4],
+                                       uint32_t sq) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float r0 = 1.f, r1 = 1.f;
   if (p.norm_w) {
     float ss0 = 0.f, ss1 = 0.f;
@@ -285,24 +221,152 @@ __global__ void __launch_bounds__(WARPS * 32, 3) diff_short_kernel(DiffParams p)
   for (int n = 0; n < W / 8; n++) {
     float2 w = make_float2(1.f, 1.f);
     if (p.norm_w) w = __ldg(reinterpret_cast<const float2*>(p.norm_w + 8 * n + 2 * t));
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at<W>(sq, row0 + g, n) + 4 * t),
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at<W>(sq, rw.row0 + g, n) + 4 * t),
                  "r"(pack2<T>(o[n][0] * r0 * w.x, o[n][1] * r0 * w.y))
                  : "memory");
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at<W>(sq, row0 + g + 8, n) + 4 * t),
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at<W>(sq, rw.row0 + g + 8, n) + 4 * t),
                  "r"(pack2<T>(o[n][2] * r1 * w.x, o[n][3] * r1 * w.y))
                  : "memory");
   }
   __syncwarp();
-  T* out = static_cast<T*>(p.out) + (long)(wh.t0 + first) * p.o_stride + (long)head * W;
+  T* out = static_cast<T*>(p.out) + (long)(wh.t0 + rw.first) * p.o_stride + (long)rw.head * W;
 #pragma unroll
   for (int e = lane; e < 16 * (W / 8); e += 32) {
     const int r = e / (W / 8), c = e % (W / 8);
     uint4 x;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                 : "r"(at<W>(sq, row0 + r, c))
+                 : "r"(at<W>(sq, rw.row0 + r, c))
                  : "memory");
-    if (first + r < wh.len) *reinterpret_cast<uint4*>(out + (long)r * p.o_stride + c * 8) = x;
+    if (rw.first + r < wh.len) *reinterpret_cast<uint4*>(out + (long)r * p.o_stride + c * 8) = x;
+  }
+}
+
+// A sequence of at most 64 tokens: every key in one block.
+template <class T, int D>
+__device__ __forceinline__ void short_rows(const DiffParams& p, const Where& wh, int lg, int head0, uint32_t sq) {
+  constexpr int W = 2 * D, TILE = 64 * W * 2;
+  const uint32_t sk = sq + TILE, sv = sk + TILE;
+  const T* q = static_cast<const T*>(p.q) + (long)wh.t0 * p.q_stride;
+  const T* k = static_cast<const T*>(p.k) + (long)wh.t0 * p.k_stride;
+  const T* v = static_cast<const T*>(p.v) + (long)wh.t0 * p.v_stride;
+  load_tile<W>(sq, q, p.q_stride, lg, wh.len, head0, p.heads, 1);
+  load_tile<W>(sk, k, p.k_stride, lg, wh.len, head0, p.heads, p.group);
+  commit_copies();
+  load_tile<W>(sv, v, p.v_stride, lg, wh.len, head0, p.heads, p.group);
+  commit_copies();
+  const Rows rw = rows_of(p, wh, lg, head0);
+  const float scale = 1.4426950408889634f * rsqrtf((float)D);
+  const float lambda = rw.work ? p.lambda[rw.head] : 0.f;
+  asm volatile("cp.async.wait_group 1;" ::: "memory");
+  __syncthreads();
+  uint32_t pa[BKEY / 16][4];
+  if (rw.work) {
+    float s[2][8][4];
+    Stat st[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      st[i].m[0] = st[i].m[1] = -INFINITY;
+      st[i].l[0] = st[i].l[1] = 0.f;
+      scores<T, D>(s[i], sq, sk, i, rw.row0, rw.key0, wh.len);
+      add_block(st[i], s[i], scale);
+    }
+    const float w1[2] = {1.f / st[0].l[0], 1.f / st[0].l[1]};
+    const float w2[2] = {lambda / st[1].l[0], lambda / st[1].l[1]};
+    weights<T>(pa, s[0], s[1], w1, w2);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  if (!rw.work) return;
+  float o[W / 8][4];
+#pragma unroll
+  for (int n = 0; n < W / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  values<T, W>(o, pa, sv, rw.key0, wh.len);
+  finish<T, W>(p, wh, rw, o, sq);
+}
+
+// Queries wh.q0 .. wh.q0 + 63 of a longer sequence and one head, in two passes
+// over the key blocks.
+template <class T, int D>
+__device__ __noinline__ void long_rows(const DiffParams& p, const Where& wh, int head0, uint32_t sq) {
+  constexpr int W = 2 * D, TILE = 64 * W * 2, lg = 6;
+  const uint32_t sk = sq + TILE, sv = sk + TILE;
+  const T* q = static_cast<const T*>(p.q) + (long)(wh.t0 + wh.q0) * p.q_stride;
+  const T* k = static_cast<const T*>(p.k) + (long)wh.t0 * p.k_stride;
+  const T* v = static_cast<const T*>(p.v) + (long)wh.t0 * p.v_stride;
+  const Rows rw = rows_of(p, wh, lg, head0);
+  const float scale = 1.4426950408889634f * rsqrtf((float)D), lambda = p.lambda[head0];
+  float o[W / 8][4];
+#pragma unroll
+  for (int n = 0; n < W / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  Stat st[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    st[i].m[0] = st[i].m[1] = -INFINITY;
+    st[i].l[0] = st[i].l[1] = 0.f;
+  }
+  load_tile<W>(sq, q, p.q_stride, lg, wh.len - wh.q0, head0, p.heads, 1);
+  for (int pass = 0; pass < 2; pass++) {
+    float w1[2], w2[2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      w1[r] = 1.f / st[0].l[r];
+      w2[r] = lambda / st[1].l[r];
+    }
+    for (int j = 0; j * BKEY < wh.len; j++) {
+      const int left = wh.len - j * BKEY;
+      load_tile<W>(sk, k + (long)j * BKEY * p.k_stride, p.k_stride, lg, left, head0, p.heads, p.group);
+      if (pass == 1) load_tile<W>(sv, v + (long)j * BKEY * p.v_stride, p.v_stride, lg, left, head0, p.heads, p.group);
+      commit_copies();
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncthreads();
+      if (rw.work) {
+        float s[2][8][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          scores<T, D>(s[i], sq, sk, i, rw.row0, 0, left);
+          if (pass == 0) {
+            add_block(st[i], s[i], scale);
+          } else {
+#pragma unroll
+            for (int n = 0; n < 8; n++)
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                s[i][n][e] = ex2f(fmaf(s[i][n][e], scale, -st[i].m[e >> 1] * scale));
+          }
+        }
+        if (pass == 1) {
+          uint32_t pa[BKEY / 16][4];
+          weights<T>(pa, s[0], s[1], w1, w2);
+          values<T, W>(o, pa, sv, 0, left);
+        }
+      }
+      __syncthreads();
+    }
+  }
+  if (rw.work) finish<T, W>(p, wh, rw, o, sq);
+}
+
+// One CTA per sequence and 64 rows of heads (of a longer sequence than the
+// kernel is for: its query blocks in turn).
+template <class T, int D>
+__global__ void __launch_bounds__(WARPS * 32, D == 64 ? 4 : 5) diff_short_kernel(const __grid_constant__ DiffParams p) {
+  pdl_wait();
+  pdl_trigger();
+  extern __shared__ __align__(128) uint8_t smem_diff[];
+  const uint32_t sq = (uint32_t)__cvta_generic_to_shared(smem_diff);
+  Where wh;
+  if (!sequence(p, p.offsets, blockIdx.x, wh) || wh.len < p.min_len || wh.len > p.max_len) return;
+  const int lg = wh.len <= 16 ? 4 : wh.len <= 32 ? 5 : 6;  // 16, 32 or 64 rows of a head in the tiles
+  const int head0 = blockIdx.y << (6 - lg);
+  if (head0 >= p.heads) return;
+  if (wh.len <= BKEY) {
+    short_rows<T, D>(p, wh, lg, head0, sq);
+    return;
+  }
+  for (; wh.q0 < wh.len; wh.q0 += BQ) {
+    long_rows<T, D>(p, wh, head0, sq);
+    __syncthreads();
   }
 }
 
@@ -324,7 +388,7 @@ static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
   }
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg =
-      pdl_config(dim3(block_count(p.T, p.nseq, BQ), p.heads), dim3(WARPS * 32), SMEM, s, attr);
+      pdl_config(dim3(p.nseq, p.heads), dim3(WARPS * 32), SMEM, s, attr);
   return cudaLaunchKernelEx(&cfg, diff_short_kernel<T, D>, p);
 }
 
