@@ -603,9 +603,7 @@ static int forward(le_model* m, const int32_t* d_ids, const int32_t* d_offsets, 
       TRY(gemm(m, 0, L.qkv, hA, H, e, s));
       if (L.head_norm) PLAUNCH(4, launch_head_norm(m, L, qkv, pos, T, s));
       if (L.diff) {
-        const DiffParams dp = diff_params(m, L, qkv, d_offsets, nseq, T, att);
-        m->prof.launches += diff_attention_launches(dp, max_len) - 1;
-        PLAUNCH(4, launch_diff_attention(DT_F16, m->head_dim, dp, max_len, s));
+        PLAUNCH(4, launch_diff_attention(DT_F16, m->head_dim, diff_params(m, L, qkv, d_offsets, nseq, T, att), max_len, s));
       } else if (att_tc)
         PLAUNCH(4, launch_attention_stc(qkv, w.att_units.p, w.cap_seqs, nseq, T, H, m->hp.heads, att,
                                         m->status.as<DevStatus>(), s));

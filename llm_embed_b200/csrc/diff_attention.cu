@@ -5,10 +5,10 @@
 // for every head, whose two query and key parts have d columns each and whose
 // values have 2d.
 //
-// For sequences of at most 64 tokens, where a call is bound by latency and by
-// how many of them are in flight: a CTA of four warps holds 64 rows of Q, K and
-// V, which are one head of up to 64 tokens, two of up to 32 or four of up to
-// 16; a warp has 16 query rows.  Both maps' scores stay in registers, so the
+// For short sequences, where a call is bound by latency, by instructions and by
+// how many sequences are in flight: a CTA of four or eight warps holds 64 or 128
+// rows of Q, K and V, which are one head of a text that long or several heads of
+// a shorter one; a warp has 16 query rows.  The scores stay in registers, so the
 // maxima and sums are known before the second product, and it runs once, on
 // P = P_1 / l_1 - lambda P_2 / l_2, rounded to the operands' type (16 bits); the
 // sums are not.  Longer sequences (a caller whose hint of the longest was too
@@ -23,7 +23,7 @@
 namespace le {
 namespace dif {
 
-constexpr int BQ = 64, BKEY = 64, WARPS = 4;
+constexpr int BKEY = 64;  // keys per block; a CTA has ROWS (64 or 128) rows and a warp for each 16
 
 template <class T>
 __device__ __forceinline__ void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
@@ -59,20 +59,20 @@ __device__ __forceinline__ uint32_t at(uint32_t base, int row, int chunk) {
   return base + row * (W * 2) + ((chunk ^ (row & 7)) << 4);
 }
 
-// 64 rows of a tile, 2^lg to a head: row r is token r % 2^lg of head r / 2^lg,
+// ROWS rows of a tile, 2^lg to a head: row r is token r % 2^lg of head r / 2^lg,
 // from src + token * ld + head * W; tokens from `n` on and heads from `heads` on
 // are zero.  `group` query heads share a head of src.  A thread keeps its chunk
 // and goes down the rows in steps whose token and head are the same for the
 // whole CTA.
-template <int W, class T>
+template <int W, int ROWS, class T>
 __device__ __forceinline__ void load_tile(uint32_t base, const T* src, long ld, int lg, int n, int head0, int heads,
                                           int group) {
-  constexpr int CH = W / 8, STEP = WARPS * 32 / CH;  // 8 or 16 rows
+  constexpr int CH = W / 8, STEP = ROWS * 2 / CH;  // rows that the CTA's threads cover: at most 2^lg
   const int r0 = threadIdx.x / CH, c = threadIdx.x % CH;
   const T* mine = src + (long)r0 * ld + c * 8;
   const uint32_t dst = at<W>(base, r0, c);
 #pragma unroll
-  for (int r = 0; r < 64; r += STEP) {
+  for (int r = 0; r < ROWS; r += STEP) {
     const int token = r & ((1 << lg) - 1), head = head0 + (r >> lg);
     const int h = group == 1 ? head : head / group;
     const bool in = token + r0 < n && head < heads;
@@ -85,7 +85,7 @@ __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_
 // Scores of a warp's 16 rows against keys key0 .. key0 + 63 of a tile (those of
 // the first `left`; -inf behind), for part `i` of the head.
 template <class T, int D>
-__device__ __forceinline__ void scores(float (&s)[8][4], uint32_t sq, uint32_t sk, int i, int row0, int key0, int left) {
+__device__ __forceinline__ void scores(float (*s)[4], uint32_t sq, uint32_t sk, int i, int row0, int key0, int left) {
   constexpr int W = 2 * D;
   const int lane = threadIdx.x & 31, t = lane & 3;
   uint32_t qa[D / 16][4];
@@ -116,11 +116,12 @@ struct Stat {
   float m[2], l[2];
 };
 
-// The block's part of the statistics; s becomes exp2(scale (s - m)).
-__device__ __forceinline__ void add_block(Stat& st, float (&s)[8][4], float scale) {
+// The part of N tiles of eight keys in the statistics; s becomes exp2(scale (s - m)).
+template <int N>
+__device__ __forceinline__ void add_block(Stat& st, float (&s)[N][4], float scale) {
   float m0 = st.m[0], m1 = st.m[1];
 #pragma unroll
-  for (int n = 0; n < 8; n++) {
+  for (int n = 0; n < N; n++) {
     m0 = fmaxf(m0, fmaxf(s[n][0], s[n][1]));
     m1 = fmaxf(m1, fmaxf(s[n][2], s[n][3]));
   }
@@ -131,7 +132,7 @@ __device__ __forceinline__ void add_block(Stat& st, float (&s)[8][4], float scal
   }
   float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-  for (int n = 0; n < 8; n++) {
+  for (int n = 0; n < N; n++) {
     s[n][0] = ex2f(fmaf(s[n][0], scale, -m0 * scale));
     s[n][1] = ex2f(fmaf(s[n][1], scale, -m0 * scale));
     s[n][2] = ex2f(fmaf(s[n][2], scale, -m1 * scale));
@@ -150,10 +151,10 @@ __device__ __forceinline__ void add_block(Stat& st, float (&s)[8][4], float scal
   st.m[1] = m1;
 }
 
-// P = w1 a - w2 b as the second product's operand.
+// P = w1 a - w2 b of 64 keys as the second product's operand.
 template <class T>
-__device__ __forceinline__ void weights(uint32_t (&pa)[BKEY / 16][4], const float (&a)[8][4], const float (&b)[8][4],
-                                        const float (&w1)[2], const float (&w2)[2]) {
+__device__ __forceinline__ void weights(uint32_t (*pa)[4], const float (*a)[4], const float (*b)[4], const float (&w1)[2],
+                                        const float (&w2)[2]) {
 #pragma unroll
   for (int n = 0; n < 8; n++) {
     pa[n / 2][2 * (n & 1)] = pack2<T>(fmaf(a[n][0], w1[0], -b[n][0] * w2[0]), fmaf(a[n][1], w1[0], -b[n][1] * w2[0]));
@@ -161,13 +162,12 @@ __device__ __forceinline__ void weights(uint32_t (&pa)[BKEY / 16][4], const floa
   }
 }
 
-// o += P V for the first `left` keys from key0.
-template <class T, int W>
-__device__ __forceinline__ void values(float (&o)[W / 8][4], const uint32_t (&pa)[BKEY / 16][4], uint32_t sv, int key0,
-                                       int left) {
+// o += P V for the first `left` of KEYS keys from key0.
+template <class T, int W, int KEYS>
+__device__ __forceinline__ void values(float (&o)[W / 8][4], const uint32_t (*pa)[4], uint32_t sv, int key0, int left) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int c = 0; c < BKEY / 16; c++)
+  for (int c = 0; c < KEYS / 16; c++)
     if (c * 16 < left) {
 #pragma unroll
       for (int n = 0; n < W / 8; n += 2) {
@@ -242,38 +242,69 @@ __device__ __forceinline__ void finish(const DiffParams& p, const Where& wh, con
   }
 }
 
-// A sequence of at most 64 tokens: every key in one block.
-template <class T, int D>
+__device__ __forceinline__ void clear(Stat& st) {
+  st.m[0] = st.m[1] = -INFINITY;
+  st.l[0] = st.l[1] = 0.f;
+}
+
+// A sequence of at most ROWS tokens: every key is in shared memory.  Of more
+// than 64 keys, the first map's weights of all keys are kept and the second
+// map's scores made twice, for its statistics and for its weights: both maps'
+// would not fit the registers.
+template <class T, int D, int ROWS>
 __device__ __forceinline__ void short_rows(const DiffParams& p, const Where& wh, int lg, int head0, uint32_t sq) {
-  constexpr int W = 2 * D, TILE = 64 * W * 2;
+  constexpr int W = 2 * D, TILE = ROWS * W * 2;
   const uint32_t sk = sq + TILE, sv = sk + TILE;
   const T* q = static_cast<const T*>(p.q) + (long)wh.t0 * p.q_stride;
   const T* k = static_cast<const T*>(p.k) + (long)wh.t0 * p.k_stride;
   const T* v = static_cast<const T*>(p.v) + (long)wh.t0 * p.v_stride;
-  load_tile<W>(sq, q, p.q_stride, lg, wh.len, head0, p.heads, 1);
-  load_tile<W>(sk, k, p.k_stride, lg, wh.len, head0, p.heads, p.group);
+  load_tile<W, ROWS>(sq, q, p.q_stride, lg, wh.len, head0, p.heads, 1);
+  load_tile<W, ROWS>(sk, k, p.k_stride, lg, wh.len, head0, p.heads, p.group);
   commit_copies();
-  load_tile<W>(sv, v, p.v_stride, lg, wh.len, head0, p.heads, p.group);
+  load_tile<W, ROWS>(sv, v, p.v_stride, lg, wh.len, head0, p.heads, p.group);
   commit_copies();
   const Rows rw = rows_of(p, wh, lg, head0);
   const float scale = 1.4426950408889634f * rsqrtf((float)D);
   const float lambda = rw.work ? p.lambda[rw.head] : 0.f;
   asm volatile("cp.async.wait_group 1;" ::: "memory");
   __syncthreads();
-  uint32_t pa[BKEY / 16][4];
+  uint32_t pa[ROWS / 16][4];
   if (rw.work) {
-    float s[2][8][4];
     Stat st[2];
+    clear(st[0]);
+    clear(st[1]);
+    if (ROWS == BKEY || wh.len <= BKEY) {
+      float s[2][8][4];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      st[i].m[0] = st[i].m[1] = -INFINITY;
-      st[i].l[0] = st[i].l[1] = 0.f;
-      scores<T, D>(s[i], sq, sk, i, rw.row0, rw.key0, wh.len);
-      add_block(st[i], s[i], scale);
+      for (int i = 0; i < 2; i++) {
+        scores<T, D>(s[i], sq, sk, i, rw.row0, rw.key0, wh.len);
+        add_block<8>(st[i], s[i], scale);
+      }
+      const float w1[2] = {1.f / st[0].l[0], 1.f / st[0].l[1]};
+      const float w2[2] = {lambda / st[1].l[0], lambda / st[1].l[1]};
+      weights<T>(pa, s[0], s[1], w1, w2);
+    } else if constexpr (ROWS > BKEY) {
+      float a[16][4], s[8][4];
+      scores<T, D>(a, sq, sk, 0, rw.row0, 0, wh.len);
+      scores<T, D>(a + 8, sq, sk, 0, rw.row0, BKEY, wh.len - BKEY);
+      add_block<16>(st[0], a, scale);
+#pragma unroll 1
+      for (int j = 0; j < 2; j++) {
+        scores<T, D>(s, sq, sk, 1, rw.row0, j * BKEY, wh.len - j * BKEY);
+        add_block<8>(st[1], s, scale);
+      }
+      const float w1[2] = {1.f / st[0].l[0], 1.f / st[0].l[1]};
+      const float w2[2] = {lambda / st[1].l[0], lambda / st[1].l[1]};
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        scores<T, D>(s, sq, sk, 1, rw.row0, j * BKEY, wh.len - j * BKEY);
+#pragma unroll
+        for (int n = 0; n < 8; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[n][e] = ex2f(fmaf(s[n][e], scale, -st[1].m[e >> 1] * scale));
+        weights<T>(pa + 4 * j, a + 8 * j, s, w1, w2);
+      }
     }
-    const float w1[2] = {1.f / st[0].l[0], 1.f / st[0].l[1]};
-    const float w2[2] = {lambda / st[1].l[0], lambda / st[1].l[1]};
-    weights<T>(pa, s[0], s[1], w1, w2);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
@@ -281,15 +312,15 @@ __device__ __forceinline__ void short_rows(const DiffParams& p, const Where& wh,
   float o[W / 8][4];
 #pragma unroll
   for (int n = 0; n < W / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  values<T, W>(o, pa, sv, rw.key0, wh.len);
+  values<T, W, ROWS>(o, pa, sv, rw.key0, wh.len);
   finish<T, W>(p, wh, rw, o, sq);
 }
 
-// Queries wh.q0 .. wh.q0 + 63 of a longer sequence and one head, in two passes
-// over the key blocks.
-template <class T, int D>
+// Queries wh.q0 .. wh.q0 + ROWS - 1 of a longer sequence and one head, in two
+// passes over blocks of ROWS keys, 64 at a time.
+template <class T, int D, int ROWS>
 __device__ __noinline__ void long_rows(const DiffParams& p, const Where& wh, int head0, uint32_t sq) {
-  constexpr int W = 2 * D, TILE = 64 * W * 2, lg = 6;
+  constexpr int W = 2 * D, TILE = ROWS * W * 2, lg = ROWS == 64 ? 6 : 7;
   const uint32_t sk = sq + TILE, sv = sk + TILE;
   const T* q = static_cast<const T*>(p.q) + (long)(wh.t0 + wh.q0) * p.q_stride;
   const T* k = static_cast<const T*>(p.k) + (long)wh.t0 * p.k_stride;
@@ -300,12 +331,9 @@ __device__ __noinline__ void long_rows(const DiffParams& p, const Where& wh, int
 #pragma unroll
   for (int n = 0; n < W / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   Stat st[2];
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    st[i].m[0] = st[i].m[1] = -INFINITY;
-    st[i].l[0] = st[i].l[1] = 0.f;
-  }
-  load_tile<W>(sq, q, p.q_stride, lg, wh.len - wh.q0, head0, p.heads, 1);
+  clear(st[0]);
+  clear(st[1]);
+  load_tile<W, ROWS>(sq, q, p.q_stride, lg, wh.len - wh.q0, head0, p.heads, 1);
   for (int pass = 0; pass < 2; pass++) {
     float w1[2], w2[2];
 #pragma unroll
@@ -313,20 +341,21 @@ __device__ __noinline__ void long_rows(const DiffParams& p, const Where& wh, int
       w1[r] = 1.f / st[0].l[r];
       w2[r] = lambda / st[1].l[r];
     }
-    for (int j = 0; j * BKEY < wh.len; j++) {
-      const int left = wh.len - j * BKEY;
-      load_tile<W>(sk, k + (long)j * BKEY * p.k_stride, p.k_stride, lg, left, head0, p.heads, p.group);
-      if (pass == 1) load_tile<W>(sv, v + (long)j * BKEY * p.v_stride, p.v_stride, lg, left, head0, p.heads, p.group);
+    for (int j = 0; j < wh.len; j += ROWS) {
+      load_tile<W, ROWS>(sk, k + (long)j * p.k_stride, p.k_stride, lg, wh.len - j, head0, p.heads, p.group);
+      if (pass == 1)
+        load_tile<W, ROWS>(sv, v + (long)j * p.v_stride, p.v_stride, lg, wh.len - j, head0, p.heads, p.group);
       commit_copies();
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncthreads();
-      if (rw.work) {
+      for (int key0 = 0; key0 < ROWS && j + key0 < wh.len && rw.work; key0 += BKEY) {
+        const int left = wh.len - j - key0;
         float s[2][8][4];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          scores<T, D>(s[i], sq, sk, i, rw.row0, 0, left);
+          scores<T, D>(s[i], sq, sk, i, rw.row0, key0, left);
           if (pass == 0) {
-            add_block(st[i], s[i], scale);
+            add_block<8>(st[i], s[i], scale);
           } else {
 #pragma unroll
             for (int n = 0; n < 8; n++)
@@ -338,7 +367,7 @@ __device__ __noinline__ void long_rows(const DiffParams& p, const Where& wh, int
         if (pass == 1) {
           uint32_t pa[BKEY / 16][4];
           weights<T>(pa, s[0], s[1], w1, w2);
-          values<T, W>(o, pa, sv, 0, left);
+          values<T, W, BKEY>(o, pa, sv, key0, left);
         }
       }
       __syncthreads();
@@ -347,32 +376,37 @@ __device__ __noinline__ void long_rows(const DiffParams& p, const Where& wh, int
   if (rw.work) finish<T, W>(p, wh, rw, o, sq);
 }
 
-// One CTA per sequence and 64 rows of heads (of a longer sequence than the
+// One CTA per sequence and ROWS rows of heads (of a longer sequence than the
 // kernel is for: its query blocks in turn).
-template <class T, int D>
-__global__ void __launch_bounds__(WARPS * 32, D == 64 ? 4 : 5) diff_short_kernel(const __grid_constant__ DiffParams p) {
+template <class T, int D, int ROWS>
+__global__ void __launch_bounds__(ROWS * 2, ROWS == 128 ? 2 : D == 64 ? 4 : 5)
+    diff_short_kernel(const __grid_constant__ DiffParams p) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ __align__(128) uint8_t smem_diff[];
   const uint32_t sq = (uint32_t)__cvta_generic_to_shared(smem_diff);
+  constexpr int TOP = ROWS == 64 ? 6 : 7;
   Where wh;
-  if (!sequence(p, p.offsets, blockIdx.x, wh) || wh.len < p.min_len || wh.len > p.max_len) return;
-  const int lg = wh.len <= 16 ? 4 : wh.len <= 32 ? 5 : 6;  // 16, 32 or 64 rows of a head in the tiles
-  const int head0 = blockIdx.y << (6 - lg);
+  if (!sequence(p, blockIdx.x, wh)) return;
+  // 16 to ROWS rows of a head in the tiles, and no fewer than one step of
+  // load_tile covers.
+  int lg = ROWS == 128 && D == 32 ? 5 : 4;
+  while (lg < TOP && wh.len > 1 << lg) lg++;
+  const int head0 = blockIdx.y << (TOP - lg);
   if (head0 >= p.heads) return;
-  if (wh.len <= BKEY) {
-    short_rows<T, D>(p, wh, lg, head0, sq);
+  if (wh.len <= ROWS) {
+    short_rows<T, D, ROWS>(p, wh, lg, head0, sq);
     return;
   }
-  for (; wh.q0 < wh.len; wh.q0 += BQ) {
-    long_rows<T, D>(p, wh, head0, sq);
+  for (; wh.q0 < wh.len; wh.q0 += ROWS) {
+    long_rows<T, D, ROWS>(p, wh, head0, sq);
     __syncthreads();
   }
 }
 
-template <class T, int D>
+template <class T, int D, int ROWS>
 static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
-  constexpr int SMEM = 3 * 64 * 2 * D * 2;
+  constexpr int SMEM = 3 * ROWS * 2 * D * 2;
   static std::mutex mu;
   static uint64_t attr_set = 0;  // per-device bit: the attribute is a per-device setting
   int dev = 0;
@@ -381,48 +415,40 @@ static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
     std::lock_guard<std::mutex> lk(mu);
     if (dev >= 64 || !(attr_set >> dev & 1)) {
       const cudaError_t e =
-          cudaFuncSetAttribute(diff_short_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+          cudaFuncSetAttribute(diff_short_kernel<T, D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
       if (e != cudaSuccess) return e;
       if (dev < 64) attr_set |= 1ull << dev;
     }
   }
   cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg =
-      pdl_config(dim3(p.nseq, p.heads), dim3(WARPS * 32), SMEM, s, attr);
-  return cudaLaunchKernelEx(&cfg, diff_short_kernel<T, D>, p);
+  const cudaLaunchConfig_t cfg = pdl_config(dim3(p.nseq, p.heads), dim3(ROWS * 2), SMEM, s, attr);
+  return cudaLaunchKernelEx(&cfg, diff_short_kernel<T, D, ROWS>, p);
+}
+template <class T, int D>
+static cudaError_t launch_rows(const DiffParams& p, int rows, cudaStream_t s) {
+  return rows == 64 ? launch<T, D, 64>(p, s) : launch<T, D, 128>(p, s);
 }
 
 }  // namespace dif
 
-static cudaError_t launch_short(int dt, int d, const DiffParams& p, cudaStream_t s) {
-  if (dt == DT_F16) return d == 64 ? dif::launch<__half, 64>(p, s) : dif::launch<__half, 32>(p, s);
-  return d == 64 ? dif::launch<__nv_bfloat16, 64>(p, s) : dif::launch<__nv_bfloat16, 32>(p, s);
+static cudaError_t launch_short(int dt, int d, const DiffParams& p, int rows, cudaStream_t s) {
+  if (dt == DT_F16) return d == 64 ? dif::launch_rows<__half, 64>(p, rows, s) : dif::launch_rows<__half, 32>(p, rows, s);
+  return d == 64 ? dif::launch_rows<__nv_bfloat16, 64>(p, rows, s) : dif::launch_rows<__nv_bfloat16, 32>(p, rows, s);
 }
 
-// Texts of at most 64 tokens: this file's kernel (256 of 16 tokens, 6 heads of
-// 64: 13 us, tcgen05 tiles 46; 256 of 64: 38 and 47).  Else the tiles (64 of 128:
-// 49 and 21 us; 256 of 16 to 128: 57 us, and 68 with the short ones taken out),
-// with the short ones taken out where nearly all are.
-enum Plan { PLAN_SHORT, PLAN_TILES, PLAN_BOTH };
-static Plan plan_of(const DiffParams& p, int max_len) {
-  if (max_len > 0 && max_len <= dif::BKEY) return PLAN_SHORT;
-  return (long)p.T < 40L * p.nseq ? PLAN_BOTH : PLAN_TILES;
-}
-int diff_attention_launches(const DiffParams& p, int max_len) {
-  return p.nseq == 0 || p.T == 0 ? 0 : plan_of(p, max_len) == PLAN_BOTH ? 2 : 1;
-}
-
-cudaError_t launch_diff_attention(int dt, int d, const DiffParams& params, int max_len, cudaStream_t s) {
-  if (params.nseq == 0 || params.T == 0) return cudaSuccess;
-  const Plan plan = plan_of(params, max_len);
-  DiffParams p = params;
-  p.min_len = 0;
-  p.max_len = plan == PLAN_BOTH ? dif::BKEY : 0x7fffffff;
-  if (plan != PLAN_TILES) {
-    const cudaError_t e = launch_short(dt, d, p, s);
-    if (e != cudaSuccess || plan == PLAN_SHORT) return e;
-    p.min_len = dif::BKEY + 1;
-  }
+// max_len, where it is known, tells the texts that this file's kernels are for;
+// they are right for others too, and slow.  Measured (us, 6 heads of 64 and 12 of
+// 32; 64 rows / 128 rows / tcgen05 tiles):
+//   256 texts of 16:        8.6 / -  / 45       8.8 / -   / 70
+//   256 of 64:              28  / 32 / 48       30  / 37  / 65
+//   256 of 30 to 70:        -   / 36 / 51       -   / 42  / 78
+//   256 of 16 to 128:       -   / 59 / 58       -   / 69  / 92
+//   256 of 128:             -   / 90 / 57       -   / 103 / 78
+cudaError_t launch_diff_attention(int dt, int d, const DiffParams& p, int max_len, cudaStream_t s) {
+  if (p.nseq == 0 || p.T == 0) return cudaSuccess;
+  if (max_len > 0 && max_len <= 64) return launch_short(dt, d, p, 64, s);
+  if (max_len > 0 && max_len <= 128 && (long)p.T < (d == 64 ? 64L : 100L) * p.nseq)
+    return launch_short(dt, d, p, 128, s);
   return launch_diff_attention_tc(dt, d, p, s);
 }
 

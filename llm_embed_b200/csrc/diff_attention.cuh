@@ -17,10 +17,10 @@ struct Where {
   int t0, len, q0;  // first row and length of the sequence, first query of the block
 };
 
-// Sequence s of `offsets`; false when it is empty or not within [0, T]
+// Sequence s; false when it is empty or not within [0, T]
 // (reported).
-__device__ __forceinline__ bool sequence(const DiffParams& p, const int32_t* offsets, int s, Where& w) {
-  const int t0 = offsets[s], t1 = offsets[s + 1];
+__device__ __forceinline__ bool sequence(const DiffParams& p, int s, Where& w) {
+  const int t0 = p.offsets[s], t1 = p.offsets[s + 1];
   if (t0 < 0 || t1 < t0 || t1 > p.T) {
     if ((threadIdx.x & 31) == 0) report(p.status, DE_BOUNDS, 80, s);
     return false;

@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       uint32_t item = blockIdx.x;
       for (uint32_t k = 0;; k++) {
         const int tile = (int)(item / (uint32_t)p.heads), head = (int)(item - (uint32_t)tile * p.heads);
-        if (tile != last) found = find_block(p, offsets, tile, BQ, w) && w.len >= p.min_len;
+        if (tile != last) found = find_block(p, offsets, tile, BQ, w);
         last = tile;
         asked = !found || w.len <= AHEAD * BKEY;
         if (asked) ask();

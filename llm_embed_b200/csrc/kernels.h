@@ -169,15 +169,12 @@ struct DiffParams {
   const float* lambda;     // [heads]
   const float* norm_w;     // [2d] or null
   float out_scale, eps;    // 1 - lambda_init
-  int min_len, max_len;    // the launch's sequences (set by launch_diff_attention)
   DevStatus* status;
 };
 // max_len: the longest sequence if known, else 0; it chooses the kernels, which
 // are right for any length.
 cudaError_t launch_diff_attention(int dt, int d, const DiffParams& p, int max_len, cudaStream_t s);
-int diff_attention_launches(const DiffParams& p, int max_len);  // kernels of such a call
-// diff_attention_tc.cu: tcgen05 tiles of 128 queries and 64 keys, sequences of
-// at least min_len tokens; the other is for at most max_len (diff_attention.cu).
+// diff_attention_tc.cu: tcgen05 tiles of 128 queries and 64 keys.
 cudaError_t launch_diff_attention_tc(int dt, int d, const DiffParams& p, cudaStream_t s);
 
 }  // namespace le

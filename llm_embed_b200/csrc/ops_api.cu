@@ -457,8 +457,7 @@ int le_diffattn_device(le_diffattn* h, const le_diffattn_args* a, void* stream) 
   p.status = h->st();
   DeviceGuard g(h->dev);
   CK(g.err);
-  const cudaStream_t s = h->pick(stream);
-  CK(launch_diff_attention(a->type, h->d, p, a->max_len, s));
+  CK(launch_diff_attention(a->type, h->d, p, a->max_len, h->pick(stream)));
   return LE_OK;
 }
 
