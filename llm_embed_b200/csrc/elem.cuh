@@ -63,6 +63,14 @@ __device__ __forceinline__ Raw8<T> load8(const T* p) {
   for (int i = 0; i < (int)(sizeof(T) / 2); i++) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
   return r;
 }
+// load8 of values that are read once (evicted first).
+template <class T>
+__device__ __forceinline__ Raw8<T> load8_once(const T* p) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 2); i++) r.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  return r;
+}
 template <class T>
 __device__ __forceinline__ Raw8<T> zero8() {
   Raw8<T> r;
@@ -96,6 +104,14 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
                                               pack2<T>(v[6], v[7]));
   }
+}
+
+// store8 of values that no kernel reads back soon.
+template <class T>
+__device__ __forceinline__ void store8_once(T* p, const float (&v)[8]) {
+  static_assert(sizeof(T) == 2, "2-byte types");
+  __stcs(reinterpret_cast<uint4*>(p), make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
+                                                 pack2<T>(v[6], v[7])));
 }
 
 }  // namespace le

@@ -6,14 +6,16 @@
 // encoder's own RoPE, ops_simd.go:127-137) or (i, i + rot/2) half-split.
 // Everything is float32 between one load and one store of each value, so a
 // result is rounded once.  Bound by memory: each head vector is read and
-// written once; the cos / sin rows and weights stay in L1 and L2.
+// written once, the cos / sin rows and weights stay in L1 and L2 (32767 tokens,
+// 32 + 8 heads of 128, bf16: 114 us, 5.9 TB/s, 0.90 of a measured copy; 18431
+// tokens, 12 + 12 heads of 64 in packed fp16 rows: 21 us, 5.3 TB/s).
 #include "elem.cuh"
 #include "kernels.h"
 
 namespace le {
 namespace qkn {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 64;
 
 // Quotient of item (< 2^30) by n; inv = floor(2^32 / n) + 1 (the high product
 // is exact or one too large).
@@ -30,7 +32,8 @@ __device__ __forceinline__ uint32_t div_by(uint32_t item, uint32_t n, uint32_t i
 // with p(i) the other column of i's pair, in the same lane (interleaved) or
 // rot/16 lanes away (half-split), whose loaded words are exchanged as they
 // are.  d is a multiple of 8, rot of 16, rows 16-byte aligned.
-template <class T, int G, int U, bool HALF>
+// ONCE: more bytes than the L2 holds, so nothing is kept there.
+template <class T, int G, int U, bool HALF, bool ONCE>
 __global__ void __launch_bounds__(THREADS) qk_norm_vec_kernel(QkNormParams p) {
   pdl_wait();
   pdl_trigger();
@@ -44,7 +47,10 @@ __global__ void __launch_bounds__(THREADS) qk_norm_vec_kernel(QkNormParams p) {
   const T* in = static_cast<const T*>(is_q ? p.q : p.k) + row * (is_q ? p.q_stride : p.k_stride) + (long)h0 * p.d + c;
   Raw8<T> raw[U];
 #pragma unroll
-  for (int u = 0; u < U; u++) raw[u] = live && h0 + u < heads ? load8(in + u * p.d) : zero8<T>();
+  for (int u = 0; u < U; u++) {
+    raw[u] = zero8<T>();
+    if (live && h0 + u < heads) raw[u] = ONCE ? load8_once(in + u * p.d) : load8(in + u * p.d);
+  }
   const int pos = item >= p.items ? -1 : p.positions ? p.positions[row] : 0;
   const bool in_table = (unsigned)pos < (unsigned)p.max_pos;
   const int lanes = p.rot / 16;  // lanes of one half of the rotated columns
@@ -117,7 +123,12 @@ __global__ void __launch_bounds__(THREADS) qk_norm_vec_kernel(QkNormParams p) {
     const float r = rsqrtf(fmaf(ss, p.inv_d, p.eps));
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = r * fmaf(v[i], A[i], o[i] * B[i]);
-    if (live && in_table && h0 + u < heads) store8(out + u * p.d, v);
+    if (live && in_table && h0 + u < heads) {
+      if constexpr (ONCE)
+        store8_once(out + u * p.d, v);
+      else
+        store8(out + u * p.d, v);
+    }
   }
   if (item < p.items && !in_table && lane == 0) report(p.status, DE_BOUNDS, 70, pos);
 }
@@ -189,25 +200,27 @@ static unsigned set_items(QkNormParams& p, int n_tokens, int U, int per_block) {
   return (p.items + per_block - 1) / per_block;
 }
 
-template <class T, int G, int U>
+template <class T, int G, int U, bool ONCE = false>
 static cudaError_t launch_vec(QkNormParams p, int n, cudaStream_t s) {
   const unsigned blocks = set_items(p, n, U, THREADS / G);
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = pdl_config(dim3(blocks), dim3(THREADS), 0, s, attr);
-  return p.half_split ? cudaLaunchKernelEx(&cfg, qk_norm_vec_kernel<T, G, U, true>, p)
-                      : cudaLaunchKernelEx(&cfg, qk_norm_vec_kernel<T, G, U, false>, p);
+  return p.half_split ? cudaLaunchKernelEx(&cfg, qk_norm_vec_kernel<T, G, U, true, ONCE>, p)
+                      : cudaLaunchKernelEx(&cfg, qk_norm_vec_kernel<T, G, U, false, ONCE>, p);
 }
 
 template <class T, int G>
 static cudaError_t launch_g(const QkNormParams& p, int n, cudaStream_t s) {
-  // Four heads per lane once that still gives every one of the 148 SMs four
+  // Four heads per lane once that still gives every one of the 148 SMs sixteen
   // blocks of them; eight of the 2-byte types where both kinds come in eights
   // (32 + 8 heads of 128, bf16: 132 -> 121 us; 12 + 12 heads of 64 padded to 16:
-  // 22.7 -> 26.4 us).
+  // 22.7 -> 26.4 us), past the L2's 126 MB with loads and stores that are not
+  // kept there (121 -> 114 us).
   const long vectors = (long)n * (p.q_heads + p.k_heads);
-  if (vectors < 148L * 4 * 4 * (THREADS / G)) return launch_vec<T, G, 1>(p, n, s);
+  if (vectors < 148L * 16 * 4 * (THREADS / G)) return launch_vec<T, G, 1>(p, n, s);
   if constexpr (sizeof(T) == 2)
-    if (p.q_heads % 8 == 0 && p.k_heads % 8 == 0) return launch_vec<T, G, 8>(p, n, s);
+    if (p.q_heads % 8 == 0 && p.k_heads % 8 == 0)
+      return 4 * vectors * p.d > 126L << 20 ? launch_vec<T, G, 8, true>(p, n, s) : launch_vec<T, G, 8>(p, n, s);
   return launch_vec<T, G, 4>(p, n, s);
 }
 
