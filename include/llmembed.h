@@ -195,16 +195,17 @@ int le_qgemm_device_noalloc(le_qweight* w, const float* d_x, int M, float* d_y, 
  * scales [ceil(K/128)][M]: the smallest power of two (>= 2^-126) that brings
  * the block's largest magnitude to 448 or less, 1 for a block of zeros, NaN
  * for one that holds a NaN or an infinity.  x / scale is exact and rounded
- * once, to nearest even.  Any M, K, stride and alignment.  On device `dev`;
- * stream NULL is its legacy default stream. */
+ * once, to nearest even.  Any M and K to 2^30, stride and alignment; q and
+ * scales may not overlap x.  On device `dev`; stream NULL is its legacy default
+ * stream. */
 int le_f8_quantize_device(int dev, int x_type, const void* d_x, int64_t ldx, int M, int K, uint8_t* d_q,
                           float* d_scales, void* stream);
 
 /* An e4m3 weight with a scale for each block of 128 x 128:
  *   y[m][n] = sum_b xs[b][m] ws[n/128][b] sum_{k in block b} xq[m][k] wq[n][k]
  * with the products of a block summed on the tensor cores and the blocks in
- * float32, rounded once to y's type.  N >= 1; K a multiple of 16 (the last
- * block may be short). */
+ * float32, rounded once to y's type.  N from 1, K a multiple of 16 (the last
+ * block may be short), M from 0, each to 2^30. */
 typedef struct le_f8weight le_f8weight;
 /* wq [N][K] bytes and scales [ceil(N/128)][ceil(K/128)] (any float32), host
  * or device memory (device: of `dev`, its contents complete). */
@@ -295,9 +296,9 @@ int le_diffattn_free(le_diffattn* h);
  * accumulated device time and launch count per kernel class.  `launches`
  * counts every kernel this library launched for the model (profiling on or
  * off).  Classes: 0 QKV GEMM, 1 attention-output GEMM, 2 FFN up/gate GEMM,
- * 3 FFN down GEMM, 4 attention (and the norm of its heads), 5 LayerNorm, 6 embedding gather + LN,
- * 7 positions + mean-pool, 8 the single-kernel forward of small calls
- * (<= 16 tokens; all layers in one launch). */
+ * 3 FFN down GEMM, 4 attention (and the norm of its heads), 5 LayerNorm,
+ * 6 embedding gather + LN, 7 positions + mean-pool, 8 the single-kernel forward
+ * of small calls (<= 16 tokens; all layers in one launch). */
 #define LE_NCLASS 9
 typedef struct {
   int64_t launches;

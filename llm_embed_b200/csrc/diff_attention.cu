@@ -117,6 +117,8 @@ struct Stat {
 };
 
 // The part of N tiles of eight keys in the statistics; s becomes exp2(scale (s - m)).
+// Scores that are all -inf so far have weight 0 (0 - 0 would be NaN), and a row
+// of nothing else ends with 0 / 0.
 template <int N>
 __device__ __forceinline__ void add_block(Stat& st, float (&s)[N][4], float scale) {
   float m0 = st.m[0], m1 = st.m[1];
@@ -130,13 +132,14 @@ __device__ __forceinline__ void add_block(Stat& st, float (&s)[N][4], float scal
     m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
     m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
   }
+  const float f0 = m0 == -INFINITY ? 0.f : m0, f1 = m1 == -INFINITY ? 0.f : m1;
   float l0 = 0.f, l1 = 0.f;
 #pragma unroll
   for (int n = 0; n < N; n++) {
-    s[n][0] = ex2f(fmaf(s[n][0], scale, -m0 * scale));
-    s[n][1] = ex2f(fmaf(s[n][1], scale, -m0 * scale));
-    s[n][2] = ex2f(fmaf(s[n][2], scale, -m1 * scale));
-    s[n][3] = ex2f(fmaf(s[n][3], scale, -m1 * scale));
+    s[n][0] = ex2f(fmaf(s[n][0], scale, -f0 * scale));
+    s[n][1] = ex2f(fmaf(s[n][1], scale, -f0 * scale));
+    s[n][2] = ex2f(fmaf(s[n][2], scale, -f1 * scale));
+    s[n][3] = ex2f(fmaf(s[n][3], scale, -f1 * scale));
     l0 += s[n][0] + s[n][1];
     l1 += s[n][2] + s[n][3];
   }
@@ -145,8 +148,8 @@ __device__ __forceinline__ void add_block(Stat& st, float (&s)[N][4], float scal
     l0 += __shfl_xor_sync(0xffffffffu, l0, o);
     l1 += __shfl_xor_sync(0xffffffffu, l1, o);
   }
-  st.l[0] = fmaf(st.l[0], ex2f((st.m[0] - m0) * scale), l0);
-  st.l[1] = fmaf(st.l[1], ex2f((st.m[1] - m1) * scale), l1);
+  st.l[0] = fmaf(st.l[0], ex2f((st.m[0] - f0) * scale), l0);
+  st.l[1] = fmaf(st.l[1], ex2f((st.m[1] - f1) * scale), l1);
   st.m[0] = m0;
   st.m[1] = m1;
 }

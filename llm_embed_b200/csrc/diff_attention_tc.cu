@@ -122,6 +122,10 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
   return e != 0;
 }
+// The maximum that weights refer to: scores that are all -inf so far have
+// weight 0 (0 - 0 would be NaN), and a row of nothing else ends with 0 / 0.
+__device__ __forceinline__ float finite(float m) { return m == -INFINITY ? 0.f : m; }
+
 template <class T, int D>
 __global__ void __launch_bounds__(NTHREADS, 1)
     diff_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (j == 0) {
           m = m0;
         } else if (__any_sync(0xffffffffu, (m0 - m) * scale > GROW)) {
-          const float f = ex2((m - m0) * scale);
+          const float f = ex2((m - finite(m0)) * scale);
           const unsigned long long f2 = f2_pack(f, f);
           // The result of the blocks before, complete.
           ok = __all_sync(0xffffffffu, mbar_wait(o_done(map), (ib - 1) & 1, abort_flag, status, 79));
@@ -455,7 +459,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             st16(to + c, w);
           }
         }
-        const unsigned long long off = f2_pack(-m * scale, -m * scale);
+        const float from = -finite(m) * scale;
+        const unsigned long long off = f2_pack(from, from);
 #pragma unroll
         for (int e = 0; e < BKEY; e += 2) {
           float x0, x1;

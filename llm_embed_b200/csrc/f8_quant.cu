@@ -87,12 +87,12 @@ __global__ void __launch_bounds__(THREADS) quant_any_kernel(const T* __restrict_
   if (lane == 0) scales[(long)kb * M + row] = s;
 }
 
-// w [N][K] float32 -> q [N][K] bytes, scales [ceil(N/128)][ceil(K/128)]: one
-// CTA per 128 x 128 block (its second read comes from L1 or L2).
-__global__ void __launch_bounds__(THREADS) quant_weight_kernel(const float* __restrict__ w, int N, int K,
+// w [N][K] float32 -> q [N][K] bytes, scales [ceil(N/128)][ceil(K/128)] (KB
+// columns): one CTA per 128 x 128 block (its second read comes from L1 or L2).
+__global__ void __launch_bounds__(THREADS) quant_weight_kernel(const float* __restrict__ w, int N, int K, int KB,
                                                                uint8_t* __restrict__ q, float* __restrict__ scales) {
   __shared__ uint32_t top;
-  const int k0 = blockIdx.x * BLOCK, n0 = blockIdx.y * BLOCK;
+  const int k0 = blockIdx.x % KB * BLOCK, n0 = blockIdx.x / KB * BLOCK;
   const int nk = min(BLOCK, K - k0), nn = min(BLOCK, N - n0);
   if (threadIdx.x == 0) top = 0;
   __syncthreads();
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(THREADS) quant_weight_kernel(const float* __re
       q[at] = (uint8_t)pack_e4m3(w[at] * inv, 0.f, 0.f, 0.f);
     }
   }
-  if (threadIdx.x == 0) scales[(long)blockIdx.y * gridDim.x + blockIdx.x] = s;
+  if (threadIdx.x == 0) scales[blockIdx.x] = s;
 }
 
 template <class T>
@@ -146,8 +146,10 @@ cudaError_t launch_f8_quantize(int dt, const void* x, long ldx, int M, int K, ui
 }
 
 cudaError_t launch_f8_quantize_weight(const float* w, int N, int K, uint8_t* q, float* scales, cudaStream_t s) {
-  const unsigned kb = (K + f8::BLOCK - 1) / f8::BLOCK, nb = (N + f8::BLOCK - 1) / f8::BLOCK;
-  f8q::quant_weight_kernel<<<dim3(kb, nb), f8q::THREADS, 0, s>>>(w, N, K, q, scales);
+  const int kb = (K + f8::BLOCK - 1) / f8::BLOCK, nb = (N + f8::BLOCK - 1) / f8::BLOCK;
+  const long blocks = (long)kb * nb;
+  if (blocks > 0x7fffffffL) return cudaErrorInvalidValue;
+  f8q::quant_weight_kernel<<<(unsigned)blocks, f8q::THREADS, 0, s>>>(w, N, K, kb, q, scales);
   return cudaGetLastError();
 }
 

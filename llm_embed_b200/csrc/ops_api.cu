@@ -121,6 +121,9 @@ int usable_device(int dev) {
 bool is_float_type(int t) { return t == LE_DT_F32 || t == LE_DT_F16 || t == LE_DT_BF16; }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+// Rows and columns of the e4m3 operators and sequences of a call: the kernels
+// count them in 32 bits, rounded up to whole tiles.
+constexpr int MAX_DIM = 1 << 30;
 
 // Frees a handle on its device, after its own stream's work.
 template <class H>
@@ -172,7 +175,7 @@ extern "C" {
 
 int le_f8_quantize_device(int dev, int x_type, const void* d_x, int64_t ldx, int M, int K, uint8_t* d_q,
                           float* d_scales, void* stream) {
-  if (M < 0 || K < 1) return le_fail(LE_EINVAL, "bad shape (M %d, K %d)", M, K);
+  if (M < 0 || K < 1 || M > MAX_DIM || K > MAX_DIM) return le_fail(LE_EINVAL, "bad shape (M %d, K %d)", M, K);
   if (!is_float_type(x_type)) return le_fail(LE_EINVAL, "x_type %d is not LE_DT_F32, LE_DT_F16 or LE_DT_BF16", x_type);
   if (ldx == 0) ldx = K;
   if (ldx < K) return le_fail(LE_EINVAL, "ldx %lld < K %d", (long long)ldx, K);
@@ -189,7 +192,8 @@ int le_f8_quantize_device(int dev, int x_type, const void* d_x, int64_t ldx, int
 
 static int f8weight_open(int dev, const void* src, int N, int K, Owner<le_f8weight>& o) {
   if (!src) return le_fail(LE_EINVAL, "null argument");
-  if (N < 1 || K < 16 || K % 16) return le_fail(LE_EINVAL, "bad shape (N %d >= 1, K %d a multiple of 16)", N, K);
+  if (N < 1 || K < 16 || K % 16 || N > MAX_DIM || K > MAX_DIM)
+    return le_fail(LE_EINVAL, "bad shape (N %d in [1, 2^30], K %d a multiple of 16 to 2^30)", N, K);
   TRY(usable_device(dev));
   if (!o.h) return le_fail(LE_ENOMEM, "out of host memory");
   return LE_OK;
@@ -248,7 +252,7 @@ static int64_t f8_work_scales_at(int64_t M, int64_t K) { return (M * K + 15) / 1
 
 int le_f8gemm_workspace(const le_f8weight* w, int M, int x_type, int64_t* bytes) {
   if (!w || !bytes) return le_fail(LE_EINVAL, "null argument");
-  if (M < 0) return le_fail(LE_EINVAL, "M < 0");
+  if (M < 0 || M > MAX_DIM) return le_fail(LE_EINVAL, "M %d outside [0, 2^30]", M);
   if (x_type != LE_DT_E4M3 && !is_float_type(x_type)) return le_fail(LE_EINVAL, "unknown x_type %d", x_type);
   *bytes = x_type == LE_DT_E4M3 ? 0 : f8_work_scales_at(M, w->K) + blocks128(w->K) * M * 4;
   return LE_OK;
@@ -425,7 +429,7 @@ int le_diffattn_create(int dev, int heads, int kv_heads, int head_dim, const flo
 int le_diffattn_device(le_diffattn* h, const le_diffattn_args* a, void* stream) {
   if (!h || !a) return le_fail(LE_EINVAL, "null argument");
   if (a->type != LE_DT_F16 && a->type != LE_DT_BF16) return le_fail(LE_EINVAL, "type %d is not LE_DT_F16 or LE_DT_BF16", a->type);
-  if (a->nseq < 0 || a->n_tokens < 0 || a->max_len < 0)
+  if (a->nseq < 0 || a->nseq > MAX_DIM || a->n_tokens < 0 || a->max_len < 0)
     return le_fail(LE_EINVAL, "bad sizes (nseq %d, tokens %d, max_len %d)", a->nseq, a->n_tokens, a->max_len);
   if (a->nseq == 0 || a->n_tokens == 0) return LE_OK;
   DiffParams p{};

@@ -69,6 +69,13 @@ def _id(table: dict, name: str, what: str) -> int:
         raise LlmEmbedError(LE_EINVAL, f"{what} {name!r} is none of {', '.join(table)}") from None
 
 
+def _i32(**sizes) -> None:
+    """Refuse sizes that a C int does not hold (ctypes would cut them)."""
+    for name, v in sizes.items():
+        if not -(1 << 31) <= v < 1 << 31:
+            raise LlmEmbedError(LE_EINVAL, f"{name} {v} does not fit 32 bits")
+
+
 def _run(fn, h, pack, stream: int, *args) -> None:
     """fn(handle, packed arguments, stream), its code checked."""
     try:
@@ -105,6 +112,7 @@ class _Handle:
 def f8_quantize_device(d_x: int, x_type: str, M: int, K: int, d_q: int, d_scales: int, ldx: int = 0, dev: int = 0,
                        stream: int = LEGACY_STREAM) -> None:
     """x [M][K] -> e4m3 bytes [M][K] and scales [ceil(K/128)][M] (le_f8_quantize_device)."""
+    _i32(M=M, K=K, dev=dev)
     rc = (_lib or lib()).le_f8_quantize_device(dev, _id(TYPES, x_type, "type"), d_x, ldx, M, K, d_q, d_scales,
                                                stream or None)
     if rc:
@@ -118,6 +126,7 @@ class F8Weight(_Handle):
 
     def __init__(self, wq, scales, N: int, K: int, dev: int = 0):
         """wq (bytes) and scales (float32): numpy arrays or host or device addresses."""
+        _i32(N=N, K=K, dev=dev)
         wp, _w = _address(wq, np.uint8, N * K)
         sp, _s = _address(scales, np.float32, -(-N // 128) * -(-K // 128))
         h = C.c_void_p()
@@ -129,6 +138,9 @@ class F8Weight(_Handle):
     def from_float(cls, w: np.ndarray, dev: int = 0) -> "F8Weight":
         """Quantise float32 w [N][K] (le_f8weight_quantize)."""
         w = np.ascontiguousarray(w, np.float32)
+        if w.ndim != 2:
+            raise LlmEmbedError(LE_EINVAL, f"w has {w.ndim} dimensions, not 2")
+        _i32(N=w.shape[0], K=w.shape[1], dev=dev)
         h = C.c_void_p()
         _check(lib().le_f8weight_quantize(dev, w.ctypes.data, w.shape[0], w.shape[1], C.byref(h)))
         self = cls.__new__(cls)
@@ -144,6 +156,7 @@ class F8Weight(_Handle):
         return q, s
 
     def workspace_bytes(self, M: int, x_type: str) -> int:
+        _i32(M=M)
         n = C.c_int64(0)
         _check(lib().le_f8gemm_workspace(self._h, M, _id(TYPES, x_type, "type"), C.byref(n)))
         return n.value
@@ -171,6 +184,7 @@ class Rope(_Handle):
     _name = "rope"
 
     def __init__(self, max_pos: int, rot_dim: int, base: float = 10000.0, pairing: str = "interleaved", dev: int = 0):
+        _i32(max_pos=max_pos, rot_dim=rot_dim, dev=dev)
         h = C.c_void_p()
         _check(lib().le_rope_create(dev, max_pos, rot_dim, base, _id(PAIRINGS, pairing, "pairing"), C.byref(h)))
         super().__init__(h)
@@ -192,6 +206,7 @@ class DiffAttention(_Handle):
     def __init__(self, heads: int, kv_heads: int, head_dim: int, lambdas, lambda_init: float, norm_weight=None,
                  eps: float = 1e-5, dev: int = 0):
         """lambdas [4][head_dim] or [heads][4][head_dim] (lq1, lk1, lq2, lk2); norm_weight [2 * head_dim] or None."""
+        _i32(heads=heads, kv_heads=kv_heads, head_dim=head_dim, dev=dev)
         lam = np.ascontiguousarray(lambdas, np.float32)
         if lam.size != 4 * head_dim and lam.size != heads * 4 * head_dim:
             raise LlmEmbedError(LE_EINVAL, f"lambdas have {lam.size} values, not [4][{head_dim}] for one or {heads} heads")
