@@ -9,12 +9,23 @@
 // holds one row's columns of one weight block, so a block costs it one
 // multiplier and half a packed fma per column.
 //
+// Bound by that addition: of about 1000 clocks a K block of 128 x 256 columns
+// costs, the tensor cores need 512 and the warps that add 256 for their fmas,
+// the rest is the way from MMA to addition and back.  Without the loads of the
+// sums it would be 121 us where it is 129 (8192 x 4096 . 4096), without the
+// wait for the accumulator 90.  Measured with rows that are quantised already:
+//   8192 x 4096 . 4096    129 us  2.13 PFLOP/s
+//   32768 x 768 . 2304     71 us  1.63 PFLOP/s
+//   512 x 4096 . 4096      15 us
+//   333 x 768 . 2304      4.8 us
+//
 // Persistent kernel; tile = 128 * CG token rows x BN weight rows.  CG = 2: a
 // cluster of two CTAs computes it with one MMA of M = 256 (cta_group::2), each
 // CTA loading its 128 token rows and half of the weight rows.
 //   warp 0     producer: TMA loads, one K block (128 bytes a row, 128B
 //              swizzle) per stage
 //   warp 1     TMEM allocation; one lane (of the even CTA) issues the MMAs
+//   warp 2     copies of the scales, three K blocks ahead
 //   warps 4-   epilogue: TMEM lanes by warp % 4, columns by group of four;
 //              rows go out through shared memory and TMA stores, or by plain
 //              stores where y's rows do not begin and end on 16 bytes
@@ -37,6 +48,7 @@ using namespace tcx;
 constexpr int BM = 128;
 constexpr int BK = 128;  // one scale block
 constexpr int EPI_WARP0 = 4;
+constexpr int SLOTS = 3, SLOT_BYTES = (BM + 4) * 4;  // K blocks whose scales are in shared memory
 
 template <int CG, int BN, int STAGES, int NACC>
 struct Cfg {
@@ -45,14 +57,17 @@ struct Cfg {
   // group has at least 64 (a 128-byte row of a 16-bit result).
   static constexpr int EPI_WARPS = BN >= 128 ? 8 : 4;
   static constexpr int COLS = BN / (EPI_WARPS / 4);  // columns of a warp
+  // Columns of a TMEM load: two loads of 32 beside 128 sums spill.
+  static constexpr int CHUNK = COLS >= 128 ? 16 : 32;
   static constexpr int NTHREADS = (EPI_WARP0 + EPI_WARPS) * 32;
   static constexpr int B_ROWS = BN / CG;  // weight rows per CTA
   static constexpr int A_BYTES = BM * BK, B_BYTES = B_ROWS * BK;
   static constexpr int OFF_A = 0;
   static constexpr int OFF_B = OFF_A + STAGES * A_BYTES;
   static constexpr int OFF_STAGE = OFF_B + STAGES * B_BYTES;
-  static constexpr int OFF_BAR = OFF_STAGE + EPI_WARPS * 2 * 4096;
-  static constexpr int NBAR = 2 * STAGES + 2 * NACC;
+  static constexpr int OFF_SCALE = OFF_STAGE + EPI_WARPS * 2 * 4096;  // [SLOTS][128 rows, up to 2 columns' groups]
+  static constexpr int OFF_BAR = OFF_SCALE + SLOTS * SLOT_BYTES;
+  static constexpr int NBAR = 2 * STAGES + 2 * NACC + 2 * SLOTS;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;
   static constexpr int TMEM_COLS = NACC * BN;
@@ -86,9 +101,9 @@ __device__ __forceinline__ void commit(uint32_t bar) {
     mma_commit(bar);
 }
 
-// 32 TMEM columns of the warp's lanes; the registers hold them after wait_ld,
-// which names them so that no use moves above it.
-__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
+// 32 or 16 TMEM columns of the warp's lanes; the registers hold them after
+// wait_ld, which names them so that no use moves above it.
+__device__ __forceinline__ void ld(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%"
       "20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -98,6 +113,13 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
 __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
@@ -105,6 +127,17 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
                  "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
                  "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
                  "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15])::"memory");
+}
+
+// acc += v * s in both halves, kept in its place between the loads and waits.
+__device__ __forceinline__ void add_scaled(unsigned long long& acc, unsigned long long v, unsigned long long s) {
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
 }
 
 // Plain stores of 32 rows x 128 bytes (words[32] of a lane: its row), turned in
@@ -164,6 +197,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
   auto empty = [&](int s) { return bar0 + 8 * (S + s); };
   auto tfull = [&](int a) { return bar0 + 8 * (2 * S + a); };
   auto tempty = [&](int a) { return bar0 + 8 * (2 * S + NACC + a); };
+  auto sfull = [&](int s) { return bar0 + 8 * (2 * S + 2 * NACC + s); };
+  auto sempty = [&](int s) { return bar0 + 8 * (2 * S + 2 * NACC + SLOTS + s); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC + 4);
 
@@ -183,6 +218,10 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     for (int a = 0; a < NACC; a++) {
       mbar_init(tfull(a), 1);
       mbar_init(tempty(a), CG * EPI_WARPS);
+    }
+    for (int s = 0; s < SLOTS; s++) {
+      mbar_init(sfull(s), 32);
+      mbar_init(sempty(s), EPI_WARPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -272,6 +311,33 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         }
       }
     }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ scales
+    // Copied ahead by a warp that has nothing else to do: a load from L2 takes
+    // as long as a K block or two, and the epilogue has no registers to wait in.
+    auto copy = [](uint32_t dst, const float* src) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+    };
+    pdl_wait();
+    uint32_t it = 0;
+    bool ok = true;
+    for (int tile = first; tile < total && ok; tile += step) {
+      // Clamped rows and columns read a scale that exists and are not stored.
+      const int row = (tile / n_tiles * CG + (int)rank) * BM + lane;
+      const float* ws = p.ws + (long)(min(tile % n_tiles * BN + lane * COLS, p.N - 1) / 128) * KB;
+      for (int kb = 0; kb < KB; kb++, it++) {
+        const int s = it % SLOTS;
+        ok = __all_sync(0xffffffffu, mbar_wait(sempty(s), ((it / SLOTS) & 1) ^ 1, abort_flag, status, 54));
+        if (!ok) break;
+        const uint32_t dst = sbase + C::OFF_SCALE + s * SLOT_BYTES + lane * 4;
+        const float* xs = p.xs + (long)kb * p.M;
+#pragma unroll
+        for (int i = 0; i < BM / 32; i++) copy(dst + i * 128, xs + min(row + 32 * i, p.M - 1));
+        if (lane < EPI_WARPS / 4) copy(dst + BM * 4, ws + kb);
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sfull(s)) : "memory");
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   } else {
     if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -284,24 +350,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     int buf = 0;
     uint32_t it = 0;
     bool ok = true;
-    // Scales are loaded two blocks ahead and multiplied when needed: a block
-    // takes less time than a load from L2.
-    const float *xs, *ws;
-    float x0 = 0.f, w0 = 0.f, x1 = 0.f, w1 = 0.f;
-    auto first_scales = [&](int tile) {
-      if (tile >= total) return;
-      // Clamped rows and columns read a scale that exists and are not stored.
-      xs = p.xs + min((tile / n_tiles * CG + (int)rank) * BM + quarter * 32 + lane, p.M - 1);
-      ws = p.ws + (long)(min(tile % n_tiles * BN + c0, p.N - 1) / 128) * KB;
-      x0 = __ldg(xs);
-      w0 = __ldg(ws);
-      if (KB > 1) {
-        x1 = __ldg(xs + p.M);
-        w1 = __ldg(ws + 1);
-      }
-    };
-    pdl_wait();  // the scales and y's memory are the previous kernels'
-    first_scales(first);
+    const float* scales = reinterpret_cast<const float*>(smem + C::OFF_SCALE);
+    pdl_wait();  // y's memory is the previous kernels'
     for (int tile = first; tile < total && ok; tile += step) {
       const int mt = tile / n_tiles, nt = tile % n_tiles;
       const int row0 = (mt * CG + (int)rank) * BM + quarter * 32, n0 = nt * BN + c0;
@@ -310,33 +360,32 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       for (int i = 0; i < COLS / 2; i++) acc[i] = 0;
       for (int kb = 0; kb < KB; kb++, it++) {
         const int a = it % NACC;
-        const float sc = x0 * w0;
-        x0 = x1;
-        w0 = w1;
-        if (kb + 2 < KB) {
-          x1 = __ldg(xs + (long)(kb + 2) * p.M);
-          w1 = __ldg(ws + kb + 2);
-        }
-        if (!__all_sync(0xffffffffu, mbar_wait(tfull(a), (it / NACC) & 1, abort_flag, status, 53))) {
+        const int s = it % SLOTS;
+        if (!__all_sync(0xffffffffu, mbar_wait(sfull(s), (it / SLOTS) & 1, abort_flag, status, 55) &&
+                                         mbar_wait(tfull(a), (it / NACC) & 1, abort_flag, status, 53))) {
           ok = false;
           break;
         }
+        const float* slot = scales + s * (SLOT_BYTES / 4);
+        const float sc = slot[quarter * 32 + lane] * slot[BM + (ew >> 2)];
         tc_fence_after();
         const unsigned long long sc2 = f2_pack(sc, sc);
         const uint32_t t = tmem + a * BN + c0 + ((uint32_t)(quarter * 32) << 16);
-        // The next 32 columns are on their way while these are added.
-        uint32_t v[2][32];
-        ld32(t, v[0]);
+        // The next columns are on their way while these are added.
+        constexpr int CH = C::CHUNK;
+        uint32_t v[2][CH];
+        ld(t, v[0]);
 #pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
-          uint32_t(&u)[32] = v[(c / 32) & 1];
+        for (int c = 0; c < COLS; c += CH) {
+          uint32_t(&u)[CH] = v[(c / CH) & 1];
           wait_ld(u);
-          if (c + 32 < COLS) {
-            ld32(t + c + 32, v[(c / 32 + 1) & 1]);
+          if (c + CH < COLS) {
+            ld(t + c + CH, v[(c / CH + 1) & 1]);
           } else {  // all read: the accumulator is free while the last columns are added
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
+              mbar_arrive(sempty(s));
               if constexpr (CG == 2)
                 mbar_arrive_cluster(map_to_rank(tempty(a), 0));
               else
@@ -344,13 +393,11 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             }
           }
 #pragma unroll
-          for (int i = 0; i < 16; i++)
-            acc[c / 2 + i] = f2_fma(f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), sc2,
-                                    acc[c / 2 + i]);
+          for (int i = 0; i < CH / 2; i++)
+            add_scaled(acc[c / 2 + i], f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), sc2);
         }
       }
       if (!ok) break;
-      first_scales(tile + step);  // on their way during the stores
       if (row0 >= p.M) continue;  // warp-uniform
       constexpr int PER = 128 / sizeof(Y);  // columns of a 128-byte block
 #pragma unroll
