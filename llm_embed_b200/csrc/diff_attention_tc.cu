@@ -18,7 +18,7 @@
 // Bound by the exponentials, two per query, key and head, 16 a clock and SM,
 // and by what they delay: instructions on barriers, TMEM and shared memory share
 // the special-function unit's queue.  16 texts of 1024 to 2047 tokens, 6 heads of
-// 64, bf16: 207 us (883 TFLOP/s; the exponentials alone 105 us at 1.9 GHz).  Of
+// 64, bf16: 204 us (897 TFLOP/s; the exponentials alone 105 us at 1.9 GHz).  Of
 // 1860 clocks that a block of 64 keys takes a map's warps, 630 are exponentials
 // (512 at least), 390 the maximum and scaling, 270 packing and writing the
 // weights, 320 the wait for scores that are ready, 170 the turn.
@@ -33,8 +33,9 @@
 //               first two blocks
 // TMEM (512 columns): two buffers of S_i / P_i for each map (64 each), O_1,
 // O_2 (2d each).  A map's MMAs run in the order they are issued - S of block
-// j + 2 after P.V of block j, whose buffer it takes - so a map has a block of
-// scores waiting while another's weights are multiplied.
+// j + 2 after P.V of block j, whose buffer it takes, also where those are blocks
+// of the next tiles - so a map has a block of scores waiting while another's
+// weights are multiplied.
 //
 // Keys past the sequence: their scores count as -inf; P.V stops at the next
 // multiple of 16 keys, and the values between (another sequence's, or
@@ -348,33 +349,53 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const uint64_t q0 = sw128_desc(sbase + L::OFF_Q + i * (D == 64 ? QTILE : 64));
       const uint64_t k0 = sw128_desc(sbase + L::OFF_K + i * (D == 64 ? KTILE : 64));
       const uint64_t v0 = (sw128_desc(sbase + L::OFF_V) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(KTILE >> 4) << 16);
-      while (ok && next_tile(n, t)) {
-        const uint32_t qs = n & 1;
-        const int nkb = (t.y + BKEY - 1) / BKEY;
-        const uint64_t qd = q0 + qs * (L::QB / 16);
-        // S of block number b, once its keys are there; then they are free,
-        // with the tile's last block the queries too.
-        auto scores = [&](uint32_t b, bool last) {
-          if (!wait(k_full(b % KV), (b / KV) & 1, 66)) return;
-          tc_fence_after();
-          if (issuer) {
-            const uint64_t kd = k0 + (b % KV) * (L::KB / 16);
-#pragma unroll
-            for (int kk = 0; kk < D / 16; kk++)
-              mma_f16(s_tm + (b & 1) * BKEY, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk != 0);
-            mma_commit(s_full(i, b));
-            mma_commit(k_empty(b % KV));
-            if (last) mma_commit(q_empty(qs));
+      // The scores run two blocks ahead of the values, into the next tiles too:
+      // S of block b + 2 goes out behind P.V of block b, whose buffer it takes.
+      uint32_t sn = 0, sb = 0;  // tiles and blocks whose scores are issued
+      bool ended = false;
+      int s_left = 0;           // blocks of the last of those tiles without scores
+      int len1 = 0, len2 = 0;   // lengths of the tiles between (at most two)
+      auto scores = [&]() {
+        if (s_left == 0) {
+          if (!next_tile(sn, t)) {
+            ended = true;
+            return;
           }
-          __syncwarp();
-        };
-        if (!wait(q_full(qs), (n >> 1) & 1, 65)) break;
-        // The scores run two blocks ahead of the values.
-        scores(ib, nkb == 1);
-        if (ok && nkb > 1) scores(ib + 1, nkb == 2);
-        if (!ok || !wait(o_empty, (n & 1) ^ 1, 68)) break;
-        for (int j = 0; j < nkb; j++, ib++) {
-          const int left = t.y - j * BKEY, steps = min(BKEY, left + 15) / 16;
+          s_left = (t.y + BKEY - 1) / BKEY;
+          if (len1 == 0)
+            len1 = t.y;
+          else
+            len2 = t.y;
+          if (!wait(q_full(sn & 1), (sn >> 1) & 1, 65)) return;
+          sn++;
+        }
+        s_left--;
+        // Once its keys are there; then they are free, with the tile's last
+        // block the queries too.
+        if (!wait(k_full(sb % KV), (sb / KV) & 1, 66)) return;
+        tc_fence_after();
+        if (issuer) {
+          const uint32_t qs = (sn - 1) & 1;
+          const uint64_t qd = q0 + qs * (L::QB / 16), kd = k0 + (sb % KV) * (L::KB / 16);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; kk++)
+            mma_f16(s_tm + (sb & 1) * BKEY, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk != 0);
+          mma_commit(s_full(i, sb));
+          mma_commit(k_empty(sb % KV));
+          if (s_left == 0) mma_commit(q_empty(qs));
+        }
+        __syncwarp();
+        sb++;
+      };
+      scores();
+      if (ok && !ended) scores();
+      while (ok && ib < sb) {
+        const int len = len1, nkb = (len + BKEY - 1) / BKEY;
+        len1 = len2;
+        len2 = 0;
+        if (!wait(o_empty, (n & 1) ^ 1, 68)) break;
+        for (int j = 0; j < nkb && ok; j++, ib++) {
+          const int left = len - j * BKEY, steps = min(BKEY, left + 15) / 16;
           if (!wait(v_full(ib % KV), (ib / KV) & 1, 67)) break;
           if (!wait(p_full(i, ib), (ib >> 1) & 1, 73)) break;
           tc_fence_after();
@@ -394,10 +415,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             if (j + 1 == nkb) mma_commit(o_full);
           }
           __syncwarp();
-          if (j + 2 < nkb) {
-            scores(ib + 2, j + 3 == nkb);
-            if (!ok) break;
-          }
+          if (!ended) scores();
         }
         n++;
       }
