@@ -154,6 +154,7 @@ struct Layer {
   DevBuf q_norm, k_norm, diff_lambda, diff_norm;
   bool head_norm = false, diff = false;
   float diff_scale = 1.f;
+  std::vector<float> diff_norm_host;
 };
 
 struct Workspace {
@@ -505,6 +506,7 @@ static DiffParams diff_params(const le_model* m, const Layer& L, const __half* q
   p.group = 1;
   p.lambda = L.diff_lambda.as<float>();
   p.norm_w = L.diff_norm.as<float>();
+  p.norm_host = L.diff_norm_host.data();
   p.out_scale = L.diff_scale;
   p.eps = m->hp.ln_eps;
   p.status = m->status.as<DevStatus>();
@@ -907,6 +909,8 @@ static int load_layer_extras(const le_model* m, Layer& L, int i, const le_tensor
     TRY(sized(dn, 2 * d));
     if (dl->type != T_F32 || dl->n_bytes < 16 * d) return fail(LE_EINVAL, "tensor %s must be F32", dl->name);
     TRY(upload_f32(L.diff_norm, dn, 2 * d, s));
+    L.diff_norm_host.resize(2 * (size_t)d);
+    std::memcpy(L.diff_norm_host.data(), dn->data, 2 * (size_t)d * 4);
     // lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init of the layer's depth.
     const double init = 0.8 - 0.6 * std::exp(-0.3 * i);
     std::vector<float> l(4 * (size_t)d);

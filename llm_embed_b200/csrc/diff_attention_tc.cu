@@ -21,7 +21,7 @@
 // 64, bf16: 204 us (897 TFLOP/s; the exponentials alone 105 us at 1.9 GHz).  Of
 // 1860 clocks that a block of 64 keys takes a map's warps, 630 are exponentials
 // (512 at least), 390 the maximum and scaling, 270 packing and writing the
-// weights, 320 the wait for scores that are ready, 170 the turn.
+// weights, 320 the wait for scores, 170 the turn.
 //
 //   warp 0      producer: TMA loads of Q (two stages), K and V (four each)
 //   warps 1, 2  MMAs of a map each: S_i = Q_i K_i^T, O_i += P_i V (one warp
@@ -44,6 +44,7 @@
 // stored.  Every mbarrier wait is bounded (WAIT_LIMIT_NS).
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "diff_attention.cuh"
@@ -62,6 +63,7 @@ constexpr int QTILE = 128 * 128, KTILE = 64 * 128;  // bytes of 128 and 64 rows 
 constexpr int KV = 4;                               // stages of K and of V
 constexpr int NTHREADS = 512;
 constexpr int RING = 4;
+constexpr int EPI = 32;  // columns of a result that the epilogue loads at a time
 constexpr int AHEAD = 8;    // tiles of more key blocks are taken one at a time
 constexpr int OFFS = 1024;  // sequences whose offsets are copied to shared memory
 constexpr float GROW = 8.f;  // log2 of the growth that moves the maximum
@@ -78,8 +80,7 @@ struct Lay {
   static constexpr int OFF_L = OFF_OUT + 4 * 4096;  // sums [2 tiles][2 maps][128]
   static constexpr int OFF_RING = OFF_L + 2 * 2 * 128 * 4;
   static constexpr int OFF_ITEM = OFF_RING + RING * 16;  // the answer that holds the next item
-  static constexpr int OFF_NORM = OFF_ITEM + 16;         // norm weights [2d]
-  static constexpr int OFF_OFFS = OFF_NORM + 2 * D * 4;
+  static constexpr int OFF_OFFS = OFF_ITEM + 16;
   static constexpr int OFF_BAR = OFF_OFFS + (OFFS + 2) * 4;
   // q_full q_empty [2 each], k_full k_empty v_full v_empty [KV each], s_full
   // p_full [2 maps][2], o_done [2], o_full o_empty, sum_full sum_empty [2 each],
@@ -99,13 +100,6 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -130,6 +124,13 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
   return e != 0;
 }
+// The norm's weights as a kernel parameter: reads from shared memory wait in the
+// queue behind the exponentials.
+template <int W>
+struct NormWeight {
+  float w[W];
+};
+
 // The maximum that weights refer to: scores that are all -inf so far have
 // weight 0 (0 - 0 would be NaN), and a row of nothing else ends with 0 / 0.
 __device__ __forceinline__ float finite(float m) { return m == -INFINITY ? 0.f : m; }
@@ -137,7 +138,8 @@ __device__ __forceinline__ float finite(float m) { return m == -INFINITY ? 0.f :
 template <class T, int D>
 __global__ void __launch_bounds__(NTHREADS, 1)
     diff_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_o, DiffParams p) {
+                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_o,
+                   const __grid_constant__ NormWeight<2 * D> norm, DiffParams p) {
   using L = Lay<D>;
   constexpr int NT = L::NT, W = 2 * D;
   constexpr uint32_t FMT = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0;
@@ -211,8 +213,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   pdl_wait();
   // No pdl_trigger: the next kernel waits for this one's CTAs, started or
   // cancelled, to be done.
-  if (threadIdx.x < W && p.norm_w) reinterpret_cast<float*>(smem + L::OFF_NORM)[threadIdx.x] = p.norm_w[threadIdx.x];
-  __syncthreads();
 
   // The next tile of the ring, for a whole warp; false at the end.
   auto next_tile = [&](uint32_t n, int4& tile) -> bool {
@@ -224,8 +224,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     return tile.y > 0;
   };
 
-  // 512 threads of 128 registers at launch; the softmax threads take what the
-  // others leave, as do the epilogue's: 56 + 2 * 144 + 168 = 4 * 128.
+  // 512 threads of 128 registers at launch: 56 + 2 * 128 + 200 = 4 * 128.  Short
+  // tiles wait for the epilogue, whose 128 results a thread and two loads of 32
+  // columns need the most (256 texts of 16 to 128: 54 us with 144 and 168
+  // registers, loads of 16 and weights in shared memory, 49 us so).
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 3) {
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
     }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     // -------------------------------------------------------------- softmax
     const int map = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -550,12 +552,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       n++;
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------------------- epilogue
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t o1 = tmem + TM_O + ((uint32_t)(quarter * 32) << 16);
     const float* sums = reinterpret_cast<const float*>(smem + L::OFF_L);
-    const float4* nw = reinterpret_cast<const float4*>(smem + L::OFF_NORM);
     const uint32_t stage = sbase + L::OFF_OUT + quarter * 4096;
     uint32_t n = 0;
     int4 t;
@@ -567,17 +568,20 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       tc_fence_after();
       const float* sum = sums + (n & 1) * 256;
       const float w1 = 1.f / sum[row], w2 = -lambda / sum[128 + row];
-      float o[W], ss = 0.f;
+      const unsigned long long w1s = f2_pack(w1, w1), w2s = f2_pack(w2, w2);
+      unsigned long long o[W / 2], ss2 = 0;
 #pragma unroll
-      for (int c = 0; c < W; c += 16) {
-        uint32_t a[16], b[16];
-        ld16(o1 + c, a);
-        ld16(o1 + W + c, b);
+      for (int c = 0; c < W; c += EPI) {
+        uint32_t a[EPI], b[EPI];
+        ld32(o1 + c, a);
+        ld32(o1 + W + c, b);
         wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          o[c + e] = fmaf(__uint_as_float(a[e]), w1, __uint_as_float(b[e]) * w2);
-          ss = fmaf(o[c + e], o[c + e], ss);
+        for (int e = 0; e < EPI; e += 2) {
+          unsigned long long& x = o[(c + e) / 2];
+          x = f2_fma(f2_pack(__uint_as_float(a[e]), __uint_as_float(a[e + 1])), w1s,
+                     f2_mul(f2_pack(__uint_as_float(b[e]), __uint_as_float(b[e + 1])), w2s));
+          ss2 = f2_fma(x, x, ss2);
         }
       }
       tc_fence_before();  // all read: the next tile's values may come
@@ -587,12 +591,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         mbar_arrive(sum_empty(n));
       }
       if (p.norm_w) {
-        const float f = p.out_scale * rsqrtf(ss * (1.f / W) + p.eps);
+        float s0, s1;
+        f2_unpack(ss2, s0, s1);
+        const float f = p.out_scale * rsqrtf((s0 + s1) * (1.f / W) + p.eps);
 #pragma unroll
-        for (int c = 0; c < W; c += 4) {
-          const float4 w = nw[c / 4];
-          o[c] *= f * w.x, o[c + 1] *= f * w.y, o[c + 2] *= f * w.z, o[c + 3] *= f * w.w;
-        }
+        for (int c = 0; c < W; c += 2) o[c / 2] = f2_mul(o[c / 2], f2_pack(f * norm.w[c], f * norm.w[c + 1]));
       }
       // 64 columns at a time; a warp whose 32 rows are all the sequence's
       // stores them through shared memory with TMA, others row by row.
@@ -601,7 +604,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       for (int c = 0; c < W; c += 64) {
         uint32_t w[32];
 #pragma unroll
-        for (int e = 0; e < 32; e++) w[e] = pack2<T>(o[c + 2 * e], o[c + 2 * e + 1]);
+        for (int e = 0; e < 32; e++) {
+          float x, y;
+          f2_unpack(o[c / 2 + e], x, y);
+          w[e] = pack2<T>(x, y);
+        }
         if (whole) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
@@ -688,7 +695,9 @@ static cudaError_t launch(const DiffParams& p, cudaStream_t s) {
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)items), dim3(NTHREADS),
                                             Lay<D>::ALLOC, s, attr);
-  return cudaLaunchKernelEx(&cfg, diff_tc_kernel<T, D>, mq, mk, mv, mo, p);
+  NormWeight<2 * D> norm = {};
+  if (p.norm_w) std::copy_n(p.norm_host, 2 * D, norm.w);
+  return cudaLaunchKernelEx(&cfg, diff_tc_kernel<T, D>, mq, mk, mv, mo, norm, p);
 }
 
 }  // namespace dtc

@@ -168,6 +168,7 @@ struct DiffParams {
   int nseq, T, heads, group;  // group: query heads per key head
   const float* lambda;     // [heads]
   const float* norm_w;     // [2d] or null
+  const float* norm_host;  // the same in host memory
   float out_scale, eps;    // 1 - lambda_init
   DevStatus* status;
 };

@@ -1,5 +1,6 @@
 // C ABI of the stand-alone operators (include/llmembed.h): handles, argument
 // checks and dispatch.
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <memory>
@@ -165,6 +166,7 @@ struct le_diffattn : OpBase {
   int heads = 0, kv_heads = 0, d = 0;
   float out_scale = 1.f, eps = 0.f;
   bool norm = false;
+  float norm_host[128] = {};
   float* lambda() const { return at<float>(0); }
   float* norm_w() const { return at<float>(step((size_t)heads * 4)); }
 };
@@ -420,6 +422,7 @@ int le_diffattn_create(int dev, int heads, int kv_heads, int head_dim, const flo
     lam[i] = (float)(std::exp(a) - std::exp(b) + (double)lambda_init);
   }
   CK(cudaMemcpy(o.h->lambda(), lam.get(), (size_t)heads * 4, cudaMemcpyHostToDevice));
+  if (norm_weight) std::copy_n(norm_weight, 2 * head_dim, o.h->norm_host);
   if (norm_weight) CK(cudaMemcpy(o.h->norm_w(), norm_weight, (size_t)2 * head_dim * 4, cudaMemcpyHostToDevice));
   CK(cudaStreamSynchronize(cudaStreamLegacy));
   *out = o.release();
@@ -456,6 +459,7 @@ int le_diffattn_device(le_diffattn* h, const le_diffattn_args* a, void* stream) 
   p.group = h->heads / h->kv_heads;
   p.lambda = h->lambda();
   p.norm_w = h->norm ? h->norm_w() : nullptr;
+  p.norm_host = h->norm_host;
   p.out_scale = h->out_scale;
   p.eps = h->eps;
   p.status = h->st();
