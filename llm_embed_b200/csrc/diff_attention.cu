@@ -442,15 +442,16 @@ static cudaError_t launch_short(int dt, int d, const DiffParams& p, int rows, cu
 // max_len, where it is known, tells the texts that this file's kernels are for;
 // they are right for others too, and slow.  Measured (us, 6 heads of 64 and 12 of
 // 32; 64 rows / 128 rows / tcgen05 tiles):
-//   256 texts of 16:        8.6 / -  / 45       8.8 / -   / 70
-//   256 of 64:              28  / 32 / 48       30  / 37  / 65
-//   256 of 30 to 70:        -   / 36 / 51       -   / 42  / 78
-//   256 of 16 to 128:       -   / 59 / 58       -   / 69  / 92
-//   256 of 128:             -   / 90 / 57       -   / 103 / 78
+//   256 texts of 16:        8.8 / -  / 39       9.0 / -   / 54
+//   256 of 64:              30  / 32 / 41       31  / 37  / 48
+//   256 of 30 to 70:        -   / 39 / 45       -   / 45  / 64
+//   256 of 40 to 90:        -   / 56 / 48       -   / 67  / 74
+//   256 of 50 to 100:       -   / 65 / 49       -   / 78  / 78
+//   256 of 128:             -   / 90 / 48       -   / 103 / 68
 cudaError_t launch_diff_attention(int dt, int d, const DiffParams& p, int max_len, cudaStream_t s) {
   if (p.nseq == 0 || p.T == 0) return cudaSuccess;
   if (max_len > 0 && max_len <= 64) return launch_short(dt, d, p, 64, s);
-  if (max_len > 0 && max_len <= 128 && (long)p.T < (d == 64 ? 64L : 100L) * p.nseq)
+  if (max_len > 0 && max_len <= 128 && (long)p.T < (d == 64 ? 56L : 75L) * p.nseq)
     return launch_short(dt, d, p, 128, s);
   return launch_diff_attention_tc(dt, d, p, s);
 }

@@ -18,10 +18,11 @@
 // Bound by the exponentials, two per query, key and head, 16 a clock and SM,
 // and by what they delay: instructions on barriers, TMEM and shared memory share
 // the special-function unit's queue.  16 texts of 1024 to 2047 tokens, 6 heads of
-// 64, bf16: 204 us (897 TFLOP/s; the exponentials alone 105 us at 1.9 GHz).  Of
+// 64, bf16: 203 us (902 TFLOP/s; the exponentials alone 105 us at 1.9 GHz).  Of
 // 1860 clocks that a block of 64 keys takes a map's warps, 630 are exponentials
 // (512 at least), 390 the maximum and scaling, 270 packing and writing the
-// weights, 320 the wait for scores, 170 the turn.
+// weights, 320 the wait for scores, 170 the turn.  256 texts of 16 to 128: 49 us;
+// the longest part of a tile of one or two key blocks is its epilogue.
 //
 //   warp 0      producer: TMA loads of Q (two stages), K and V (four each)
 //   warps 1, 2  MMAs of a map each: S_i = Q_i K_i^T, O_i += P_i V (one warp
