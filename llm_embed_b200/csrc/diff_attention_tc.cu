@@ -301,7 +301,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n}\n"
             : "=r"(more), "=&r"(item)
             : "l"(lo), "l"(hi));
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read before the next answer
+        // Every lane has read the answer before lane 0 asks for the next one,
+        // which overwrites it.
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
         if (!more) break;
       }
       if (ok) publish(make_int4(0, 0, 0, 0));

@@ -878,3 +878,25 @@ def test_attention_layer(lens):
     del g
     for hnd in (qkv_w, out_w, rope, attn):
         hnd.close()
+
+
+@gpu
+@pytest.mark.parametrize("heads", [1, 16])
+@pytest.mark.parametrize("count", [900, 1500])
+def test_diff_attention_mostly_empty_sequences(heads, count):
+    """Tiles without rows among short ones: a CTA asks for its next tile again
+    and again with nothing published between, several heads of one lookup."""
+    import torch
+    d = 64
+    lens = [(s % 7 == 3) * (1 + s % 90) for s in range(count)]
+    q, k, v, offs, t = make_diff(lens, heads, heads, d, "f16", count)
+    lam, val = lambdas(heads, d, True, 3)
+    a = ops.DiffAttention(heads, heads, d, lam, INIT, None)
+    out = run_diff(a, q, k, v, offs, t, heads, d, "f16", 0)
+    a.sync()
+    for _ in range(5):
+        assert torch.equal(out, run_diff(a, q, k, v, offs, t, heads, d, "f16", 0))
+    a.sync()
+    ref, mag = diff64(q, k, v, offs.tolist(), heads, heads, d, val, INIT, None, 0)
+    check_diff(out, ref, mag, "f16")
+    a.close()
