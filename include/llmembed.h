@@ -285,7 +285,8 @@ typedef struct {
   int32_t max_len;         /* longest sequence if known, else 0: only chooses the kernel */
 } le_diffattn_args;
 /* Offsets that descend or leave [0, n_tokens] are reported by
- * le_diffattn_sync; their sequences are not computed. */
+ * le_diffattn_sync; no row outside [0, n_tokens) is then read or written, but
+ * which rows of the call's other sequences are computed is not defined. */
 int le_diffattn_device(le_diffattn* h, const le_diffattn_args* a, void* stream);
 int le_diffattn_sync(le_diffattn* h);
 int le_diffattn_free(le_diffattn* h);

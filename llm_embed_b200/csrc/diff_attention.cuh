@@ -65,9 +65,9 @@ __device__ __forceinline__ bool find_block(const DiffParams& p, const int32_t* o
   return true;
 }
 
-// Reports offsets that descend or leave [0, T] (one CTA of a launch runs it).
-__device__ __forceinline__ void check_offsets(const DiffParams& p, int nthreads) {
-  for (int s = threadIdx.x; s < p.nseq; s += nthreads) {
+// Reports offsets that descend or leave [0, T] (one warp of a launch runs it).
+__device__ __forceinline__ void check_offsets(const DiffParams& p) {
+  for (int s = threadIdx.x & 31; s < p.nseq; s += 32) {
     const int a = p.offsets[s], b = p.offsets[s + 1];
     if (a < 0 || b < a || b > p.T) report(p.status, DE_BOUNDS, 81, s);
   }

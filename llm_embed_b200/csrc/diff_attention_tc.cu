@@ -233,7 +233,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 3) {
       // -------------------------------------------------------------- tiles
-      if (blockIdx.x == 0) check_offsets(p, 32);
       uint32_t n = 0;
       auto publish = [&](int4 t) -> bool {
         const int e = n % RING;
@@ -279,6 +278,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       uint32_t item = blockIdx.x;
       for (uint32_t k = 0;; k++) {
         const int tile = (int)(item / (uint32_t)p.heads), head = (int)(item - (uint32_t)tile * p.heads);
+        if (item == 0) check_offsets(p);  // whichever CTA has it: the first may itself be cancelled
         if (tile != last) found = find_block(p, offsets, tile, BQ, w);
         last = tile;
         asked = !found || w.len <= AHEAD * BKEY;

@@ -900,3 +900,31 @@ def test_diff_attention_mostly_empty_sequences(heads, count):
     ref, mag = diff64(q, k, v, offs.tolist(), heads, heads, d, val, INIT, None, 0)
     check_diff(out, ref, mag, "f16")
     a.close()
+
+
+@gpu
+@pytest.mark.parametrize("hint", [0, 1, 100])
+@pytest.mark.parametrize("bad", [[0, 300, 200, 400], [0, 300, 401], [-128, 0, 400], [0, 399, 0, 400], [400, 0, 400],
+                                 [0, 2 ** 31 - 1, 128, 400], [0] * 50 + [300, 200] + [400] * 50])
+def test_diff_attention_bad_offsets_of_any_kernel(bad, hint):
+    """Every kernel reports them, also where no tile begins with the sequence
+    that descends (the first list: numbers 0, 3 and 3), and writes only rows of
+    the batch; the next call is as ever."""
+    import torch
+    h, d, t = 2, 64, 400
+    q, k, v, _, _ = make_diff([t], h, h, d, "f16", 1)
+    lam, val = lambdas(h, d, False, 2)
+    a = ops.DiffAttention(h, h, d, lam, INIT, None)
+    out = torch.full((t + 260, 2 * h * d), 7.0, device="cuda", dtype=torch.float16)
+    o = torch.tensor(bad, dtype=torch.int32, device="cuda")
+    a.run_device("f16", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), len(bad) - 1, t, hint,
+                 out[130].data_ptr(), q_stride=q.stride(0), k_stride=k.stride(0), v_stride=v.stride(0), stream=stream())
+    with pytest.raises(LlmEmbedError) as e:
+        a.sync()
+    assert e.value.code == -3
+    assert (out[:130] == 7).all() and (out[130 + t:] == 7).all()
+    good = np.array([0, 250, 400], np.int32)
+    ref, mag = diff64(q, k, v, good.tolist(), h, h, d, val, INIT, None, 0)
+    check_diff(run_diff(a, q, k, v, good, t, h, d, "f16", hint), ref, mag, "f16")
+    a.sync()
+    a.close()
