@@ -10,13 +10,14 @@
 // rows of Q, K and V, which are one head of a text that long or several heads of
 // a shorter one; a warp has 16 query rows.  The scores stay in registers, so the
 // maxima and sums are known before the second product, and it runs once, on
-// P = P_1 / l_1 - lambda P_2 / l_2, rounded to the operands' type (16 bits); the
-// sums are not.  Longer sequences (a caller whose hint of the longest was too
+// P = P_1 / l_1 - lambda P_2 / l_2, rounded to the operands' type (16 bits, in
+// the upper part of fp16's range); the sums are not.  Longer sequences (a caller whose hint of the longest was too
 // small) take the same steps block by block, in two passes: maxima and sums,
 // then weights and values.
 // Keys past the sequence get weight 0 and their values are zeros in shared
 // memory, whatever the rows behind hold.
 #include <mutex>
+#include <type_traits>
 
 #include "diff_attention.cuh"
 
@@ -154,6 +155,23 @@ __device__ __forceinline__ void add_block(Stat& st, float (&s)[N][4], float scal
   st.m[1] = m1;
 }
 
+// The power of two that P is multiplied by before its rounding, and the result
+// divided by: P is at most 1 + |lambda| and as small as 1 / keys, and fp16 has all
+// its bits from 2^-14 to 2^16 only, so P goes up to 2^15 and a bit; bf16 needs
+// nothing.  Powers of two change no other rounding.
+template <class T>
+struct Lift {
+  float up = 1.f, down = 1.f;
+  __device__ __forceinline__ explicit Lift(float lambda) {
+    if constexpr (std::is_same<T, __half>::value) {
+      // 2^(14 - e) with 2^e <= max(1, |lambda|) < 2^(e + 1): P below 3 * 2^14
+      const uint32_t e = (__float_as_uint(fmaxf(fabsf(lambda), 1.f)) >> 23) - 127;
+      up = __uint_as_float((127 + 14 - e) << 23);
+      down = __uint_as_float((127 - 14 + e) << 23);
+    }
+  }
+};
+
 // P = w1 a - w2 b of 64 keys as the second product's operand.
 template <class T>
 __device__ __forceinline__ void weights(uint32_t (*pa)[4], const float (*a)[4], const float (*b)[4], const float (&w1)[2],
@@ -197,13 +215,14 @@ __device__ __forceinline__ Rows rows_of(const DiffParams& p, const Where& wh, in
   return r;
 }
 
-// Norm, then out through the warp's own rows of the query tile: whole 16-byte
+// Scaled back (down) and normed, then out through the warp's own rows of the query tile: whole 16-byte
 // chunks of a row instead of pairs of elements.
 template <class T, int W>
 __device__ __forceinline__ void finish(const DiffParams& p, const Where& wh, const Rows& rw, float (&o)[W / 8][4],
                                        uint32_t sq) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float r0 = 1.f, r1 = 1.f;
+  const float down = Lift<T>(__ldg(p.lambda + rw.head)).down;  // not held since the weights
+  float r0 = down, r1 = down;
   if (p.norm_w) {
     float ss0 = 0.f, ss1 = 0.f;
 #pragma unroll
@@ -216,8 +235,8 @@ __device__ __forceinline__ void finish(const DiffParams& p, const Where& wh, con
       ss0 += __shfl_xor_sync(0xffffffffu, ss0, e);
       ss1 += __shfl_xor_sync(0xffffffffu, ss1, e);
     }
-    r0 = p.out_scale * rsqrtf(ss0 / (float)W + p.eps);
-    r1 = p.out_scale * rsqrtf(ss1 / (float)W + p.eps);
+    r0 *= p.out_scale * rsqrtf(ss0 * (down * down) / (float)W + p.eps);
+    r1 *= p.out_scale * rsqrtf(ss1 * (down * down) / (float)W + p.eps);
   }
   __syncwarp();
 #pragma unroll
@@ -269,6 +288,7 @@ __device__ __forceinline__ void short_rows(const DiffParams& p, const Where& wh,
   const Rows rw = rows_of(p, wh, lg, head0);
   const float scale = 1.4426950408889634f * rsqrtf((float)D);
   const float lambda = rw.work ? p.lambda[rw.head] : 0.f;
+  const Lift<T> lift(lambda);
   asm volatile("cp.async.wait_group 1;" ::: "memory");
   __syncthreads();
   uint32_t pa[ROWS / 16][4];
@@ -283,8 +303,8 @@ __device__ __forceinline__ void short_rows(const DiffParams& p, const Where& wh,
         scores<T, D>(s[i], sq, sk, i, rw.row0, rw.key0, wh.len);
         add_block<8>(st[i], s[i], scale);
       }
-      const float w1[2] = {1.f / st[0].l[0], 1.f / st[0].l[1]};
-      const float w2[2] = {lambda / st[1].l[0], lambda / st[1].l[1]};
+      const float w1[2] = {lift.up / st[0].l[0], lift.up / st[0].l[1]};
+      const float w2[2] = {lift.up * lambda / st[1].l[0], lift.up * lambda / st[1].l[1]};
       weights<T>(pa, s[0], s[1], w1, w2);
     } else if constexpr (ROWS > BKEY) {
       float a[16][4], s[8][4];
@@ -296,8 +316,8 @@ __device__ __forceinline__ void short_rows(const DiffParams& p, const Where& wh,
         scores<T, D>(s, sq, sk, 1, rw.row0, j * BKEY, wh.len - j * BKEY);
         add_block<8>(st[1], s, scale);
       }
-      const float w1[2] = {1.f / st[0].l[0], 1.f / st[0].l[1]};
-      const float w2[2] = {lambda / st[1].l[0], lambda / st[1].l[1]};
+      const float w1[2] = {lift.up / st[0].l[0], lift.up / st[0].l[1]};
+      const float w2[2] = {lift.up * lambda / st[1].l[0], lift.up * lambda / st[1].l[1]};
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         scores<T, D>(s, sq, sk, 1, rw.row0, j * BKEY, wh.len - j * BKEY);
@@ -330,6 +350,7 @@ __device__ __noinline__ void long_rows(const DiffParams& p, const Where& wh, int
   const T* v = static_cast<const T*>(p.v) + (long)wh.t0 * p.v_stride;
   const Rows rw = rows_of(p, wh, lg, head0);
   const float scale = 1.4426950408889634f * rsqrtf((float)D), lambda = p.lambda[head0];
+  const Lift<T> lift(lambda);
   float o[W / 8][4];
 #pragma unroll
   for (int n = 0; n < W / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -341,8 +362,8 @@ __device__ __noinline__ void long_rows(const DiffParams& p, const Where& wh, int
     float w1[2], w2[2];
 #pragma unroll
     for (int r = 0; r < 2; r++) {
-      w1[r] = 1.f / st[0].l[r];
-      w2[r] = lambda / st[1].l[r];
+      w1[r] = lift.up / st[0].l[r];
+      w2[r] = lift.up * lambda / st[1].l[r];
     }
     for (int j = 0; j < wh.len; j += ROWS) {
       load_tile<W, ROWS>(sk, k + (long)j * p.k_stride, p.k_stride, lg, wh.len - j, head0, p.heads, p.group);

@@ -928,3 +928,79 @@ def test_diff_attention_bad_offsets_of_any_kernel(bad, hint):
     check_diff(run_diff(a, q, k, v, good, t, h, d, "f16", hint), ref, mag, "f16")
     a.sync()
     a.close()
+
+
+def sink_and_small_weights(n, d, name):
+    """One head of n keys: key 0 takes nearly all of both maps and has no value,
+    the others' weights lie near 2^-20 and 2^-19; and the exact result."""
+    import torch
+    q = torch.zeros(n, 2 * d, device="cuda")
+    k, v = torch.zeros_like(q), torch.randn(n, 2 * d, device="cuda", generator=gen(n)).abs()
+    q[:, 0], q[:, d] = 8, 8
+    k[0, 0], k[0, d] = math.log(2) * 20 * math.sqrt(d) / 8, math.log(2) * 19 * math.sqrt(d) / 8
+    k[1:, 1::2] = 0.1 * torch.randn(n - 1, d, device="cuda", generator=gen(n + 1))
+    v[0] = 0
+    return [x.to(T(name)) for x in (q, k, v)]
+
+
+@gpu
+@pytest.mark.parametrize("n,hint", [(16, 16), (60, 60), (100, 100), (128, 128), (100, 1), (1000, 1), (1000, 100)])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [32, 64])
+@pytest.mark.parametrize("norm", [True, False])
+def test_diff_attention_small_weights(n, hint, name, d, norm):
+    """Weights far below the row's largest keep their half step: the formula's
+    tolerance holds where fp16's own range (2^-14) would not give it."""
+    q, k, v = sink_and_small_weights(n, d, name)
+    offs = np.array([0, n] + [n] * (n // 8), np.int32)  # short on average
+    nw = np.linspace(0.5, 1.5, 2 * d).astype(np.float32) if norm else None
+    lam, val = lambdas(1, d, True, 2)
+    a = ops.DiffAttention(1, 1, d, lam, INIT, nw, 1e-20)
+    import torch
+    ref, mag = diff64(q, k, v, offs.tolist(), 1, 1, d, val, INIT, None if nw is None else torch.from_numpy(nw).cuda(), 1e-20)
+    out = run_diff(a, q, k, v, offs, n, 1, d, name, hint)
+    a.sync()
+    # Scores reach 20 log 2 = 14: their sums have at most two terms, off by
+    # 2^-24 of 14, which check_diff's 2^-13 covers.
+    check_diff(out, ref, mag, name)
+    a.close()
+
+
+@gpu
+@pytest.mark.parametrize("n,hint", [(9, 9), (60, 60), (100, 100), (300, 1)])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_diff_attention_large_lambda(n, hint, name):
+    """A lambda past fp16's largest value: the weights' difference stays in range."""
+    import torch
+    h, d = 2, 64
+    q, k, v, offs, t = make_diff([n] + [0] * n, h, h, d, name, n)
+    lam = np.zeros((4, d), np.float32)
+    lam[0, 0], lam[1, 0] = 4, 3  # exp(12) = 162755
+    val = [math.exp(12.0) - 1 + INIT] * h
+    nw = np.ones(2 * d, np.float32)
+    a = ops.DiffAttention(h, h, d, lam, INIT, nw, 1e-5)
+    ref, mag = diff64(q, k, v, offs.tolist(), h, h, d, val, INIT, torch.from_numpy(nw).cuda(), 1e-5)
+    out = run_diff(a, q, k, v, offs, t, h, d, name, hint)
+    a.sync()
+    assert torch.isfinite(ref).all()
+    check_diff(out, ref, mag, name)
+    a.close()
+
+
+@gpu
+@pytest.mark.parametrize("hint", [0, 1])
+def test_diff_attention_flat_rows_of_many_keys(hint):
+    """Equal scores over 65536 keys: (1 - lambda) times the mean value, with
+    weights of 5e-6 (85.47 of fp16's smallest steps) where they are divided
+    by their sums first."""
+    import torch
+    n, d = 65536, 32
+    q = torch.zeros(n, 2 * d, device="cuda", dtype=torch.float16)
+    k, v = torch.ones_like(q), (1 + 0.25 * torch.randn(n, 2 * d, device="cuda", generator=gen(1))).half()
+    a = ops.DiffAttention(1, 1, d, np.zeros((4, d), np.float32), INIT, None)
+    out = run_diff(a, q, k, v, np.array([0, n], np.int32), n, 1, d, "f16", hint)
+    a.sync()
+    mean, mag = v.double().mean(0), v.double().abs().mean(0)
+    ref = ((1 - INIT) * mean).expand(n, -1)
+    check_diff(out, ref, ((1 + INIT) * mag).expand(n, -1), "f16")
+    a.close()
