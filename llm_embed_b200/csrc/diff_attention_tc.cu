@@ -11,9 +11,10 @@
 // one query row (TMEM lane): it reads the 64 scores of a key block, writes
 // the weights back over them as 16-bit pairs (the A operand of P.V), and keeps
 // the row's maximum and sum.  The maximum that the weights refer to is only
-// moved when it has grown by more than 2^8 (the weights then stay below 2^8,
-// far inside the operand's range, and the sums are float32), so rescaling the
-// result in TMEM is rare.
+// moved when it has grown by more than 2^8 (the weights then stay within 2^8 of
+// its own, inside the operand's range, and the sums are float32), so rescaling
+// the result in TMEM is rare.  The weights are the only values rounded to 16 bits
+// before the result: the tensor cores take no wider operand at their rate.
 //
 // Bound by the exponentials, two per query, key and head, 16 a clock and SM,
 // and by what they delay: instructions on barriers, TMEM and shared memory share
@@ -47,6 +48,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "diff_attention.cuh"
 #include "gemm_epi_tc.cuh"
@@ -68,6 +70,12 @@ constexpr int EPI = 32;  // columns of a result that the epilogue loads at a tim
 constexpr int AHEAD = 8;    // tiles of more key blocks are taken one at a time
 constexpr int OFFS = 1024;  // sequences whose offsets are copied to shared memory
 constexpr float GROW = 8.f;  // log2 of the growth that moves the maximum
+// log2 of the weight of a score at that maximum.  fp16 has all its bits from
+// 2^-14 to 2^16 only, so its weights go up to 2^15 and those down to 2^-21 of the
+// maximum's keep their 11 bits; bf16 has the range of float32.  The sums are of
+// the same scale, so the result does not know of it.
+template <class T>
+constexpr float LIFT = std::is_same<T, __half>::value ? 15.f - GROW : 0.f;
 
 template <int D>
 struct Lay {
@@ -490,7 +498,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             st16(to + c, w);
           }
         }
-        const float from = -finite(m) * scale;
+        const float from = fmaf(-finite(m), scale, LIFT<T>);
         const unsigned long long off = f2_pack(from, from);
 #pragma unroll
         for (int e = 0; e < BKEY; e += 2) {

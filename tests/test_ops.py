@@ -1004,3 +1004,41 @@ def test_diff_attention_flat_rows_of_many_keys(hint):
     ref = ((1 - INIT) * mean).expand(n, -1)
     check_diff(out, ref, ((1 + INIT) * mag).expand(n, -1), "f16")
     a.close()
+
+
+@gpu
+@pytest.mark.parametrize("n", [16, 100, 1000, 5000])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [32, 64])
+def test_diff_attention_small_weights_in_tiles(n, name, d):
+    """test_diff_attention_small_weights for the tiles of longer texts."""
+    q, k, v = sink_and_small_weights(n, d, name)
+    offs = np.array([0, n], np.int32)
+    lam, val = lambdas(1, d, True, 2)
+    a = ops.DiffAttention(1, 1, d, lam, INIT, None)
+    ref, mag = diff64(q, k, v, [0, n], 1, 1, d, val, INIT, None, 0)
+    out = run_diff(a, q, k, v, offs, n, 1, d, name, 0)
+    a.sync()
+    check_diff(out, ref, mag, name)
+    a.close()
+
+
+@gpu
+def test_diff_attention_tiles_largest_weights():
+    """fp16 weights past the maximum they refer to: scores that grow by less
+    than what moves it, up to 2^8 times the first block's."""
+    import torch
+    n, d = 640, 64
+    q = torch.zeros(n, 2 * d, device="cuda")
+    k, v = torch.zeros_like(q), torch.randn(n, 2 * d, device="cuda", generator=gen(3))
+    q[:, 0], q[:, d] = 8, 8
+    k[:, 0] = torch.arange(n, device="cuda") // 64 * 0.61  # 9 * 0.61 = 5.49, 2^7.92
+    k[:, d] = 5.5 * (torch.arange(n, device="cuda") >= 64)
+    q, k, v = q.half(), k.half(), v.half()
+    lam, val = lambdas(1, d, True, 2)
+    a = ops.DiffAttention(1, 1, d, lam, INIT, None)
+    ref, mag = diff64(q, k, v, [0, n], 1, 1, d, val, INIT, None, 0)
+    out = run_diff(a, q, k, v, np.array([0, n], np.int32), n, 1, d, "f16", 0)
+    a.sync()
+    check_diff(out, ref, mag, "f16")
+    a.close()
