@@ -5,10 +5,12 @@ position rotation (Rope), and differential attention (DiffAttention).
 
 As with embed.QWeight the calls take device addresses, enqueue their work on
 `stream` and return; the formulas, shapes and limits are in
-include/llmembed.h.  `stream` 0 is the handle's own stream, which does not
-order with the legacy default stream; pass LEGACY_STREAM for that one (a
-framework whose current stream has the handle 0 means it).  Element types are
-"f32", "f16", "bf16" and "e4m3".
+include/llmembed.h.  Without a `stream` all of them go to the legacy default
+stream, so one call's result may be the next one's input (a framework whose
+current stream has the handle 0 means that one: pass LEGACY_STREAM).  `stream` 0
+is the handle's own stream (the quantiser has no handle: the legacy one), which
+orders neither with that nor with another handle's.  Element types are "f32",
+"f16", "bf16" and "e4m3".
 """
 from __future__ import annotations
 
@@ -163,7 +165,7 @@ class F8Weight(_Handle):
 
     def matmul_device(self, d_x: int, M: int, d_y: int, x_type: str = "f16", y_type: str = "f16", ldx: int = 0,
                       ldy: int = 0, d_x_scales: int = 0, d_work: int = 0, work_bytes: int = 0,
-                      stream: int = 0) -> None:
+                      stream: int = LEGACY_STREAM) -> None:
         """y [M][N] = x [M][K] . W^T; x is quantised in the call, or e4m3 with d_x_scales."""
         _run((_lib or lib()).le_f8gemm_device, self._h, _F8GEMM_ARGS, stream, d_x, d_x_scales, d_y, d_work, work_bytes,
              ldx, ldy, M, _id(TYPES, x_type, "type"), _id(TYPES, y_type, "type"))
@@ -192,7 +194,7 @@ class Rope(_Handle):
     def qk_norm_device(self, dtype: str, n_tokens: int, q_heads: int, k_heads: int, head_dim: int, d_q: int, d_k: int,
                        d_positions: int, d_q_out: int, d_k_out: int, q_stride: int = 0, k_stride: int = 0,
                        q_out_stride: int = 0, k_out_stride: int = 0, d_q_weight: int = 0, d_k_weight: int = 0,
-                       eps: float = 1e-6, stream: int = 0) -> None:
+                       eps: float = 1e-6, stream: int = LEGACY_STREAM) -> None:
         _run((_lib or lib()).le_qk_norm_device, self._h, _QK_NORM_ARGS, stream, d_q, d_k, d_q_out, d_k_out, d_q_weight,
              d_k_weight, d_positions, q_stride, k_stride, q_out_stride, k_out_stride, _id(TYPES, dtype, "type"),
              n_tokens, q_heads, k_heads, head_dim, eps)
@@ -220,6 +222,6 @@ class DiffAttention(_Handle):
 
     def run_device(self, dtype: str, d_q: int, d_k: int, d_v: int, d_offsets: int, nseq: int, n_tokens: int,
                    max_len: int, d_out: int, q_stride: int = 0, k_stride: int = 0, v_stride: int = 0,
-                   out_stride: int = 0, stream: int = 0) -> None:
+                   out_stride: int = 0, stream: int = LEGACY_STREAM) -> None:
         _run((_lib or lib()).le_diffattn_device, self._h, _DIFFATTN_ARGS, stream, d_q, d_k, d_v, d_out, d_offsets,
              q_stride, k_stride, v_stride, out_stride, _id(TYPES, dtype, "type"), nseq, n_tokens, max_len)

@@ -1042,3 +1042,47 @@ def test_diff_attention_tiles_largest_weights():
     a.sync()
     check_diff(out, ref, mag, "f16")
     a.close()
+
+
+# ----------------------------------------------------------------- streams --
+
+def test_operators_share_one_default_stream():
+    """One call's result is the next one's input: without a stream of the
+    caller's all of them go to the same."""
+    import inspect
+    calls = (ops.f8_quantize_device, ops.F8Weight.matmul_device, ops.Rope.qk_norm_device, ops.DiffAttention.run_device)
+    assert [inspect.signature(c).parameters["stream"].default for c in calls] == [ops.LEGACY_STREAM] * 4
+
+
+@gpu
+def test_default_streams_are_ordered():
+    """Quantiser, product, head norm and attention without a stream argument,
+    behind work on the legacy stream that takes a while."""
+    import torch
+    t, h, d = 40, 2, 64
+    W = 2 * h * d
+    w8, ws = make_f8(3 * W, W, 1)
+    w = ops.F8Weight(w8.data_ptr(), ws.data_ptr(), 3 * W, W)
+    rope = ops.Rope(t, d)
+    a = ops.DiffAttention(h, h, d, np.zeros((4, d), np.float32), INIT)
+    pos = torch.arange(t, device="cuda", dtype=torch.int32)
+    offs = torch.tensor([0, t], device="cuda", dtype=torch.int32)
+    x = torch.randn(t, W, device="cuda", generator=gen(2)).half()
+
+    def layer(**kw):
+        q, s = torch.zeros(t, W, device="cuda", dtype=torch.uint8), torch.zeros(-(-W // 128), t, device="cuda")
+        qkv, out = (torch.zeros(t, n, device="cuda", dtype=torch.float16) for n in (3 * W, W))
+        torch.cuda.synchronize()
+        torch.cuda._sleep(20_000_000)  # 10 ms on the legacy stream
+        ops.f8_quantize_device(x.data_ptr(), "f16", t, W, q.data_ptr(), s.data_ptr(), **kw)
+        w.matmul_device(q.data_ptr(), t, qkv.data_ptr(), "e4m3", "f16", d_x_scales=s.data_ptr(), **kw)
+        pq, pk, pv = (qkv.data_ptr() + 2 * W * i for i in range(3))
+        rope.qk_norm_device("f16", t, 2 * h, 2 * h, d, pq, pk, pos.data_ptr(), pq, pk, 3 * W, 3 * W, 3 * W, 3 * W, **kw)
+        a.run_device("f16", pq, pk, pv, offs.data_ptr(), 1, t, t, out.data_ptr(), 3 * W, 3 * W, 3 * W, **kw)
+        torch.cuda.synchronize()
+        return out
+
+    want = layer(stream=ops.LEGACY_STREAM)  # and loads the kernels, which waits for the device
+    assert torch.equal(layer(), want)
+    for hnd in (w, rope, a):
+        hnd.close()
