@@ -78,7 +78,17 @@ int le_init(int* ndev);
 
 /* Upload one full model replica to device `dev` and repack its weights into
  * the tile-blocked layout.  Replaces LoadBertModel + PreDequant +
- * NewRoPETable (bert.go:91, bert.go:542, embedder.go:26-29). */
+ * NewRoPETable (bert.go:91, bert.go:542, embedder.go:26-29).
+ * Optional F32 tensors of a layer that the reference does not know (dims in
+ * GGUF order; LE_EINVAL when one of a pair is missing or has another size):
+ *   blk.N.attn_q_norm.weight, attn_k_norm.weight [head_dim]: norm of the query
+ *     and key heads (le_qk_norm_device) with ln_eps, before the rotation;
+ *   blk.N.attn_diff_lambda.weight [head_dim, 4] (lq1, lk1, lq2, lk2 one after
+ *     another), attn_diff_norm.weight [2 head_dim]: differential attention
+ *     (le_diffattn_device) of pairs of heads, lambda_init 0.8 - 0.6 exp(-0.3 N).
+ * attn_q_norm / attn_k_norm with a bias, or with one weight for each of the
+ * `hidden` columns, are another operator's and are not read, like any other
+ * tensor without a use here. */
 int le_model_load(int dev, const le_tensor_desc* tensors, int n_tensors, const le_hparams* hp, le_model** out);
 
 /* Convenience: parse a GGUF file (GGUF v2/v3, 32-byte data alignment as

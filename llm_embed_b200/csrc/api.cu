@@ -887,12 +887,21 @@ static const le_tensor_desc* find(const le_tensor_desc* t, int nt, const std::st
 static int load_layer_extras(const le_model* m, Layer& L, int i, const le_tensor_desc* ts, int nt, cudaStream_t s) {
   const std::string p = "blk." + std::to_string(i) + ".";
   const int d = m->head_dim;
-  auto sized = [&](const le_tensor_desc* t, int64_t n) {
+  auto elements = [](const le_tensor_desc* t) {
     int64_t have = 1;
-    for (int k = 0; k < t->n_dims; k++) have *= t->dims[k];
+    for (int k = 0; k < t->n_dims && k < 4; k++) have *= t->dims[k];
+    return have;
+  };
+  auto sized = [&](const le_tensor_desc* t, int64_t n) {
+    const int64_t have = elements(t);
     return have == n ? LE_OK : fail(LE_EINVAL, "%s has %lld elements, expected %lld", t->name, (long long)have, (long long)n);
   };
   const le_tensor_desc *qn = find(ts, nt, p + "attn_q_norm.weight"), *kn = find(ts, nt, p + "attn_k_norm.weight");
+  // Norms with a bias or of whole rows are another operator's tensors: not read,
+  // like every other tensor that the reference does not know.
+  bool other = find(ts, nt, p + "attn_q_norm.bias") || find(ts, nt, p + "attn_k_norm.bias");
+  for (const le_tensor_desc* t : {qn, kn}) other = other || (t && d != m->hp.hidden && elements(t) == m->hp.hidden);
+  if (other) qn = kn = nullptr;
   if (!qn != !kn) return fail(LE_EINVAL, "%sattn_q_norm.weight and attn_k_norm.weight come together", p.c_str());
   if (qn) {
     TRY(sized(qn, d));

@@ -130,3 +130,32 @@ def test_tensors_come_together_and_fit(model_path):
             with pytest.raises(LlmEmbedError) as err:
                 load(change)
             assert err.value.code == LE_EINVAL
+
+
+def embed_tensors(ts, spec, ids, offs):
+    hp = HParams(n_layers=spec.layers, hidden=spec.hidden, ffn=spec.ffn, heads=spec.heads, context_length=spec.context,
+                 ln_eps=spec.eps, rope_base=spec.rope_base)
+    e = Embedder.LoadTensors([(n, *x) for n, x in ts.items()], hp)
+    try:
+        return e.EmbedIDs(ids, offs)
+    finally:
+        e.Close()
+
+
+@pytest.mark.parametrize("size,bias", [("row", True), ("row", False), ("head", True)])
+def test_norms_of_another_kind_are_not_read(model_path, size, bias):
+    """Norms of whole query and key rows, or with a bias, are another operator
+    than the heads' norm: a model that has them gives what it does without, as
+    in the reference, which knows no such tensors."""
+    spec = spec_of(False, False)
+    _, tensors = synth.read_gguf(model_path(spec))
+    ids, offs = synth.make_ids([30, 1, 17], seed=7, vocab=spec.vocab)
+    ts = {n: (t, list(dims), bytes(b)) for n, (t, dims, b) in tensors.items()}
+    want = embed_tensors(ts, spec, ids, offs)
+    n = spec.hidden if size == "row" else spec.hidden // spec.heads
+    for i in range(spec.layers):
+        for name in ("attn_q_norm", "attn_k_norm"):
+            ts[f"blk.{i}.{name}.weight"] = (synth.GGML_F32, [n], np.full(n, 1.5, np.float32).tobytes())
+            if bias:
+                ts[f"blk.{i}.{name}.bias"] = (synth.GGML_F32, [n], np.full(n, 0.5, np.float32).tobytes())
+    assert np.array_equal(embed_tensors(ts, spec, ids, offs), want)
