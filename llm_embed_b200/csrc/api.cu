@@ -915,6 +915,9 @@ static int load_layer_extras(const le_model* m, Layer& L, int i, const le_tensor
   if (dl) {
     if (m->hp.heads % 2) return fail(LE_EINVAL, "differential attention needs an even number of heads (%d)", m->hp.heads);
     TRY(sized(dl, 4 * d));
+    // lq1, lk1, lq2, lk2 one after another: [head_dim, 4] in GGUF order, or flat.
+    if (dl->dims[0] != d && dl->dims[0] != 4 * d)
+      return fail(LE_EINVAL, "%s has rows of %lld values, expected %d", dl->name, (long long)dl->dims[0], d);
     TRY(sized(dn, 2 * d));
     if (dl->type != T_F32 || dl->n_bytes < 16 * d) return fail(LE_EINVAL, "tensor %s must be F32", dl->name);
     TRY(upload_f32(L.diff_norm, dn, 2 * d, s));

@@ -159,3 +159,23 @@ def test_norms_of_another_kind_are_not_read(model_path, size, bias):
             if bias:
                 ts[f"blk.{i}.{name}.bias"] = (synth.GGML_F32, [n], np.full(n, 0.5, np.float32).tobytes())
     assert np.array_equal(embed_tensors(ts, spec, ids, offs), want)
+
+
+@pytest.mark.parametrize("dims,fits", [([64, 4], True), ([256], True), ([4, 64], False), ([128, 2], False)])
+def test_lambda_layout(model_path, dims, fits):
+    """The learned weights are four vectors of head_dim one after another; the
+    same number of values in another layout is refused."""
+    spec = spec_of(False, True)
+    _, tensors = synth.read_gguf(model_path(spec))
+    ids, offs = synth.make_ids([9], seed=7, vocab=spec.vocab)
+    ts = {n: (t, list(d), bytes(b)) for n, (t, d, b) in tensors.items()}
+    want = embed_tensors(ts, spec, ids, offs)
+    for i in range(spec.layers):
+        t, _, b = ts[f"blk.{i}.attn_diff_lambda.weight"]
+        ts[f"blk.{i}.attn_diff_lambda.weight"] = (t, dims, b)
+    if fits:
+        assert np.array_equal(embed_tensors(ts, spec, ids, offs), want)
+    else:
+        with pytest.raises(LlmEmbedError) as err:
+            embed_tensors(ts, spec, ids, offs)
+        assert err.value.code == LE_EINVAL
