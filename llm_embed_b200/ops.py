@@ -174,9 +174,10 @@ class F8Weight(_Handle):
 def _address(a, dtype, n: int):
     if isinstance(a, int):
         return a, None
-    a = np.ascontiguousarray(a).view(dtype) if np.asarray(a).dtype.itemsize == np.dtype(dtype).itemsize else None
-    if a is None or a.size != n:
-        raise LlmEmbedError(LE_EINVAL, f"expected {n} values of {np.dtype(dtype).name}")
+    a, dtype = np.ascontiguousarray(a), np.dtype(dtype)
+    # Bytes may be of any type of one byte; other values are what they are.
+    if a.dtype != dtype and (a.dtype.itemsize != 1 or dtype.itemsize != 1) or a.size != n:
+        raise LlmEmbedError(LE_EINVAL, f"expected {n} values of {dtype.name}, not {a.size} of {a.dtype.name}")
     return a.ctypes.data, a
 
 
@@ -210,6 +211,8 @@ class DiffAttention(_Handle):
         """lambdas [4][head_dim] or [heads][4][head_dim] (lq1, lk1, lq2, lk2); norm_weight [2 * head_dim] or None."""
         _i32(heads=heads, kv_heads=kv_heads, head_dim=head_dim, dev=dev)
         lam = np.ascontiguousarray(lambdas, np.float32)
+        if heads < 1 or head_dim < 1:
+            raise LlmEmbedError(LE_EINVAL, f"heads {heads} and head_dim {head_dim} must be positive")
         if lam.size != 4 * head_dim and lam.size != heads * 4 * head_dim:
             raise LlmEmbedError(LE_EINVAL, f"lambdas have {lam.size} values, not [4][{head_dim}] for one or {heads} heads")
         nw = None if norm_weight is None else np.ascontiguousarray(norm_weight, np.float32)

@@ -1086,3 +1086,14 @@ def test_default_streams_are_ordered():
     assert torch.equal(layer(), want)
     for hnd in (w, rope, a):
         hnd.close()
+
+
+def test_refusals_of_array_types():
+    """Scales in another type are refused, not reinterpreted; sizes of zero."""
+    w = np.zeros((16, 16), np.uint8)
+    for bad in (np.ones((1, 1), np.int32), np.ones((1, 1), np.uint32), np.ones((1, 1), np.float16)):
+        expect_einval(lambda: ops.F8Weight(w, bad, 16, 16))
+    for bad in (w.astype(np.float32), w.astype(np.uint16), w[:, :8]):
+        expect_einval(lambda: ops.F8Weight(bad, np.ones((1, 1), np.float32), 16, 16))
+    expect_einval(lambda: ops.DiffAttention(1, 1, 0, np.zeros(0, np.float32), 0.8))
+    expect_einval(lambda: ops.DiffAttention(0, 1, 64, np.zeros((0, 4, 64), np.float32), 0.8))
