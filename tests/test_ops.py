@@ -1097,3 +1097,29 @@ def test_refusals_of_array_types():
         expect_einval(lambda: ops.F8Weight(bad, np.ones((1, 1), np.float32), 16, 16))
     expect_einval(lambda: ops.DiffAttention(1, 1, 0, np.zeros(0, np.float32), 0.8))
     expect_einval(lambda: ops.DiffAttention(0, 1, 64, np.zeros((0, 4, 64), np.float32), 0.8))
+
+
+@gpu
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,rot", [(64, 16), (128, 96), (50, 20), (64, 0)])
+@pytest.mark.parametrize("pairing", ["interleaved", "half"])
+def test_qk_norm_infinite_values(name, d, rot, pairing):
+    """A head with an infinity has norm factor 0: the infinity's own column (with
+    the rotation, its pair) is NaN, every other one 0, whichever kernel."""
+    import torch
+    t = 2 * d
+    q = torch.randn(t, 2 * d, device="cuda", generator=gen(d)).to(T(name))
+    for i in range(d):
+        q[i, i] = float("inf")
+        q[d + i, i] = float("-inf")
+    pos = torch.arange(t, device="cuda", dtype=torch.int32)
+    out = torch.empty_like(q)
+    r = ops.Rope(t, rot, 10000.0, pairing)
+    r.qk_norm_device(name, t, 2, 0, d, q.data_ptr(), 0, pos.data_ptr(), out.data_ptr(), 0, stream=stream())
+    r.sync()
+    ref = qk64(q, 2, d, rot, pairing, None, pos, 10000.0, 1e-6)
+    got = out.double().reshape(ref.shape)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    assert int(torch.isnan(ref[:, 0]).sum()) == 2 * d + 2 * rot and (got[:, 0].nan_to_num(0) == 0).all()
+    check_qk(out.reshape(ref.shape)[:, 1:], ref[:, 1:], name)
+    r.close()
