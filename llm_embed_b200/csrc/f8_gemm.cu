@@ -22,6 +22,7 @@ namespace f8s {
 using namespace f8;
 
 constexpr int ROWS = 16;  // weight rows per CTA
+constexpr int WARPS = 8;
 
 struct E4m3 {};  // activations that are quantised already
 
@@ -94,85 +95,71 @@ struct Act<E4m3> {
   }
 };
 
-// NT groups of eight tokens, RT tiles of 16 weight rows per CTA, DEPTH K
-// blocks of each warp in flight.
-template <class X, class Y, int NT, int RT, int DEPTH, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) f8_small_kernel(F8GemmParams p) {
-  __shared__ float red[WARPS][NT * 8][RT * ROWS + 1];
+// NT groups of eight tokens.
+template <class X, class Y, int NT>
+__global__ void __launch_bounds__(WARPS * 32, 2) f8_small_kernel(F8GemmParams p) {
+  __shared__ float red[WARPS][NT * 8][ROWS + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * (RT * ROWS), m0 = blockIdx.y * (8 * NT);
+  const int n0 = blockIdx.x * ROWS, m0 = blockIdx.y * (8 * NT);
   const int KB = (p.K + BLOCK - 1) / BLOCK;
   const float* ws = p.ws + (long)(n0 / BLOCK) * KB;
   const uint8_t* wrow = p.w + (long)(n0 + g) * p.K;
-  uint4 w[DEPTH][2 * RT][2];
-  float wsc[DEPTH];
-  // Rows g, g + 8, .. of block kb: two pieces of 16 bytes each.
-  auto load_w = [&](int d, int kb) {
+  uint4 w[2][2];
+  float wsc;
+  // Rows g and g + 8 of block kb: two pieces of 16 bytes each.
+  auto load_w = [&](int kb) {
 #pragma unroll
-    for (int r = 0; r < 2 * RT; r++)
+    for (int r = 0; r < 2; r++)
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         const int k = kb * BLOCK + 64 * c + 16 * t;
-        w[d][r][c] = ldw(wrow + (long)(8 * r) * p.K + k, n0 + g + 8 * r < p.N && k < p.K);
+        w[r][c] = ldw(wrow + (long)(8 * r) * p.K + k, n0 + g + 8 * r < p.N && k < p.K);
       }
-    wsc[d] = kb < KB ? __ldg(ws + kb) : 0.f;
+    wsc = kb < KB ? __ldg(ws + kb) : 0.f;
   };
   // The weight is no other kernel's result, so its first blocks are under way
   // before the previous kernel (the quantiser, if there is one) has ended.
-#pragma unroll
-  for (int d = 0; d < DEPTH; d++) load_w(d, warp + d * WARPS);
+  load_w(warp);
   pdl_wait();
   pdl_trigger();
-  float acc[RT][NT][4];
+  float acc[NT][4];
 #pragma unroll
-  for (int r = 0; r < RT; r++)
+  for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  for (int kb = warp; kb < KB; kb += WARPS) {
+    Act<X> x[NT];
 #pragma unroll
-    for (int j = 0; j < NT; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0.f;
-  for (int kb0 = warp; kb0 < KB; kb0 += WARPS * DEPTH) {
-    Act<X> x[DEPTH][NT];
-#pragma unroll
-    for (int d = 0; d < DEPTH; d++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) x[d][j].load(p, m0 + 8 * j + g, kb0 + d * WARPS, t);
-#pragma unroll
-    for (int d = 0; d < DEPTH; d++) {
-#pragma unroll
-      for (int j = 0; j < NT; j++) {
-        uint32_t f[8];
-        const float xs = x[d][j].frag(f);
-        // Columns 2t and 2t + 1 of the result: the scales of those tokens.
-        const float s0 = __shfl_sync(0xffffffffu, xs, 8 * t) * wsc[d];
-        const float s1 = __shfl_sync(0xffffffffu, xs, 8 * t + 4) * wsc[d];
-#pragma unroll
-        for (int r = 0; r < RT; r++) {
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 2; c++) {
-            const uint4 a = w[d][2 * r][c], b = w[d][2 * r + 1][c];
-            mma_e4m3(v, a.x, b.x, a.y, b.y, f[4 * c], f[4 * c + 1]);
-            mma_e4m3(v, a.z, b.z, a.w, b.w, f[4 * c + 2], f[4 * c + 3]);
-          }
-          acc[r][j][0] = fmaf(v[0], s0, acc[r][j][0]);
-          acc[r][j][1] = fmaf(v[1], s1, acc[r][j][1]);
-          acc[r][j][2] = fmaf(v[2], s0, acc[r][j][2]);
-          acc[r][j][3] = fmaf(v[3], s1, acc[r][j][3]);
-        }
-      }
-      load_w(d, kb0 + (DEPTH + d) * WARPS);
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < RT; r++)
+    for (int j = 0; j < NT; j++) x[j].load(p, m0 + 8 * j + g, kb, t);
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-      red[warp][8 * j + 2 * t][r * ROWS + g] = acc[r][j][0];
-      red[warp][8 * j + 2 * t + 1][r * ROWS + g] = acc[r][j][1];
-      red[warp][8 * j + 2 * t][r * ROWS + g + 8] = acc[r][j][2];
-      red[warp][8 * j + 2 * t + 1][r * ROWS + g + 8] = acc[r][j][3];
+      uint32_t f[8];
+      const float xs = x[j].frag(f);
+      // Columns 2t and 2t + 1 of the result: the scales of those tokens.
+      const float s0 = __shfl_sync(0xffffffffu, xs, 8 * t) * wsc;
+      const float s1 = __shfl_sync(0xffffffffu, xs, 8 * t + 4) * wsc;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const uint4 a = w[0][c], b = w[1][c];
+        mma_e4m3(v, a.x, b.x, a.y, b.y, f[4 * c], f[4 * c + 1]);
+        mma_e4m3(v, a.z, b.z, a.w, b.w, f[4 * c + 2], f[4 * c + 3]);
+      }
+      acc[j][0] = fmaf(v[0], s0, acc[j][0]);
+      acc[j][1] = fmaf(v[1], s1, acc[j][1]);
+      acc[j][2] = fmaf(v[2], s0, acc[j][2]);
+      acc[j][3] = fmaf(v[3], s1, acc[j][3]);
     }
+    load_w(kb + WARPS);
+  }
+#pragma unroll
+  for (int j = 0; j < NT; j++) {
+    red[warp][8 * j + 2 * t][g] = acc[j][0];
+    red[warp][8 * j + 2 * t + 1][g] = acc[j][1];
+    red[warp][8 * j + 2 * t][g + 8] = acc[j][2];
+    red[warp][8 * j + 2 * t + 1][g + 8] = acc[j][3];
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < NT * 8 * RT * ROWS; i += WARPS * 32) {
-    const int m = i / (RT * ROWS), n = i % (RT * ROWS);
+  for (int i = threadIdx.x; i < NT * 8 * ROWS; i += WARPS * 32) {
+    const int m = i / ROWS, n = i % ROWS;
     float v = red[0][m][n];
 #pragma unroll
     for (int k = 1; k < WARPS; k++) v += red[k][m][n];
@@ -180,21 +167,21 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) f8_small_kernel(F8Gemm
   }
 }
 
-template <class X, class Y, int NT, int RT, int DEPTH, int WARPS>
+template <class X, class Y, int NT>
 static cudaError_t launch_nt(const F8GemmParams& p, cudaStream_t s) {
   cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg = pdl_config(
-      dim3((p.N + RT * ROWS - 1) / (RT * ROWS), (p.M + 8 * NT - 1) / (8 * NT)), dim3(WARPS * 32), 0, s, attr);
-  return cudaLaunchKernelEx(&cfg, f8_small_kernel<X, Y, NT, RT, DEPTH, WARPS>, p);
+  const cudaLaunchConfig_t cfg =
+      pdl_config(dim3((p.N + ROWS - 1) / ROWS, (p.M + 8 * NT - 1) / (8 * NT)), dim3(WARPS * 32), 0, s, attr);
+  return cudaLaunchKernelEx(&cfg, f8_small_kernel<X, Y, NT>, p);
 }
 template <class X, class Y>
 static cudaError_t launch_xy(const F8GemmParams& p, cudaStream_t s) {
   if constexpr (sizeof(X) == 1) {
-    if (p.M > 24) return launch_nt<X, Y, 4, 1, 1, 8>(p, s);
-    if (p.M > 16) return launch_nt<X, Y, 3, 1, 1, 8>(p, s);
-    if (p.M > 8) return launch_nt<X, Y, 2, 1, 1, 8>(p, s);
+    if (p.M > 24) return launch_nt<X, Y, 4>(p, s);
+    if (p.M > 16) return launch_nt<X, Y, 3>(p, s);
+    if (p.M > 8) return launch_nt<X, Y, 2>(p, s);
   }
-  return launch_nt<X, Y, 1, 1, 1, 8>(p, s);
+  return launch_nt<X, Y, 1>(p, s);
 }
 template <class X>
 static cudaError_t launch_x(int ydt, const F8GemmParams& p, cudaStream_t s) {
