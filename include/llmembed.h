@@ -236,6 +236,9 @@ typedef struct {
 } le_f8gemm_args;
 /* Bytes of workspace that a call with M rows of x_type needs (0 for e4m3). */
 int le_f8gemm_workspace(const le_f8weight* w, int M, int x_type, int64_t* bytes);
+/* Weight rows in one tile of the kernel that a call with M rows of x and N
+ * weight rows takes: 16 (few rows), 64, 128 or 256 (a pair of CTAs). */
+int le_f8gemm_tile(int M, int N);
 /* y = x . W^T.  x of LE_DT_F32/F16/BF16 is quantised within the call (any
  * alignment and stride); x of LE_DT_E4M3 is taken as it is, 16-byte aligned
  * with ldx a multiple of 16. */

@@ -527,18 +527,24 @@ using Tile64 = Cfg<1, 64, 8, 4>;
 
 template <class Y>
 static cudaError_t pick(int ydt, const F8GemmParams& p, DevStatus* status, cudaStream_t s) {
-  // Measured cost of one wave of tiles, 64 : 128 : 256 wide, about 4 : 5 : 8
-  // (K = 768: 4.1, 5.0 and 6.6 us, K = 4096: 10.4, 13.6 and 20 us).
-  const long sms = 148, m1 = (p.M + 127) / 128, m2 = (m1 + 1) / 2;
-  auto waves = [](long tiles, long slots) { return (tiles + slots - 1) / slots; };
-  const long c64 = 4 * waves(m1 * ((p.N + 63) / 64), sms), c128 = 5 * waves(m1 * ((p.N + 127) / 128), sms),
-             c256 = 8 * waves(m2 * ((p.N + 255) / 256), sms / 2);
-  if (c256 <= c128 && c256 <= c64) return launch<Pair, Y>(ydt, p, status, s);
-  if (c128 <= c64) return launch<Tile128, Y>(ydt, p, status, s);
-  return launch<Tile64, Y>(ydt, p, status, s);
+  switch (f8_tile(p.M, p.N)) {
+    case 256: return launch<Pair, Y>(ydt, p, status, s);
+    case 128: return launch<Tile128, Y>(ydt, p, status, s);
+    default: return launch<Tile64, Y>(ydt, p, status, s);
+  }
 }
 
 }  // namespace f8t
+
+int f8_tile(int M, int N) {
+  // Measured cost of one wave of tiles, 64 : 128 : 256 wide, about 4 : 5 : 8
+  // (K = 768: 4.1, 5.0 and 6.6 us, K = 4096: 10.4, 13.6 and 20 us).
+  const long sms = 148, m1 = ((long)M + 127) / 128, m2 = (m1 + 1) / 2, n = N;
+  auto waves = [](long tiles, long slots) { return (tiles + slots - 1) / slots; };
+  const long c64 = 4 * waves(m1 * ((n + 63) / 64), sms), c128 = 5 * waves(m1 * ((n + 127) / 128), sms),
+             c256 = 8 * waves(m2 * ((n + 255) / 256), sms / 2);
+  return c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
+}
 
 cudaError_t launch_f8_gemm_tc(int ydt, const F8GemmParams& p, DevStatus* status, cudaStream_t s) {
   if (p.M == 0) return cudaSuccess;

@@ -156,7 +156,8 @@ struct F8GemmParams {
 constexpr int F8_SMALL_MAX_M = 32;  // f8_gemm.cu's most rows; F8_FUSED_MAX_M: of x that is not e4m3
 constexpr int F8_FUSED_MAX_M = 8;
 cudaError_t launch_f8_gemm_small(int xdt, int ydt, const F8GemmParams& p, cudaStream_t s);
-// f8_gemm_tc.cu: e4m3 activations, tcgen05 tiles.
+// f8_gemm_tc.cu: e4m3 activations, tcgen05 tiles f8_tile weight rows wide.
+int f8_tile(int M, int N);
 cudaError_t launch_f8_gemm_tc(int ydt, const F8GemmParams& p, DevStatus* status, cudaStream_t s);
 
 // diff_attention.cu: differential attention over packed sequences.

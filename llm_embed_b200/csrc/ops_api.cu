@@ -260,6 +260,8 @@ int le_f8gemm_workspace(const le_f8weight* w, int M, int x_type, int64_t* bytes)
   return LE_OK;
 }
 
+int le_f8gemm_tile(int M, int N) { return M <= 0 || N <= 0 ? 0 : M <= F8_SMALL_MAX_M ? 16 : f8_tile(M, N); }
+
 int le_f8gemm_device(le_f8weight* w, const le_f8gemm_args* a, void* stream) {
   if (!w || !a) return le_fail(LE_EINVAL, "null argument");
   F8GemmParams p{};

@@ -52,6 +52,7 @@ def lib() -> C.CDLL:
                 L.le_f8weight_quantize.argtypes = [i, vp, i, i, out]
                 L.le_f8weight_read.argtypes = [vp, vp, vp]
                 L.le_f8gemm_workspace.argtypes = [vp, i, i, C.POINTER(i64)]
+                L.le_f8gemm_tile.argtypes = [i, i]
                 L.le_f8gemm_device.argtypes = [vp, vp, vp]
                 L.le_rope_create.argtypes = [i, i, i, C.c_double, i, out]
                 L.le_qk_norm_device.argtypes = [vp, vp, vp]

@@ -1123,3 +1123,101 @@ def test_qk_norm_infinite_values(name, d, rot, pairing):
     assert int(torch.isnan(ref[:, 0]).sum()) == 2 * d + 2 * rot and (got[:, 0].nan_to_num(0) == 0).all()
     check_qk(out.reshape(ref.shape)[:, 1:], ref[:, 1:], name)
     r.close()
+
+
+# ------------------------------------------------- products of many tiles --
+
+# (m, k, n, ldy, tile): more tiles than run at once, several K blocks and a short
+# last one, rows that end inside a tile or (4097) fill one CTA of a pair only,
+# y rows that TMA stores take and (ldy or n not on 16 bytes) plain ones.
+MANY_TILES = [(4225, 784, 2312, 0, 256), (4097, 784, 2296, 0, 256), (4225, 784, 2310, 0, 256),
+              (4300, 2064, 2312, 2315, 256), (4352, 16, 2560, 0, 256), (4225, 128, 2311, 0, 256),
+              (8000, 128, 1032, 1033, 128),
+              (33000, 400, 257, 0, 128), (20000, 784, 72, 0, 128), (19500, 784, 128, 131, 128), (20000, 16, 120, 0, 128),
+              (20000, 784, 64, 0, 64), (40000, 400, 40, 0, 64), (40000, 784, 33, 37, 64), (40000, 16, 48, 0, 64)]
+
+
+def test_products_of_many_tiles_take_the_tile_they_are_for():
+    for m, _, n, _, tile in MANY_TILES:
+        assert ops.lib().le_f8gemm_tile(m, n) == tile, (m, n)
+    assert [ops.lib().le_f8gemm_tile(m, 768) for m in (0, 1, 32, 33)] == [0, 16, 16, 64]
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n,ldy,tile", MANY_TILES)
+@pytest.mark.parametrize("xt,yt", [("f16", "f16"), ("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])
+def test_product_many_tiles(m, k, n, ldy, tile, xt, yt):
+    """A CTA takes several tiles: stages, accumulators and scales go on from one
+    to the next; a NaN stays in its row, and twice gives the same bits."""
+    import torch
+    w8, ws = make_f8(n, k, m)
+    x = (torch.randn(m, k, device="cuda", generator=gen(k)) * torch.exp(
+        torch.randn(m, 1, device="cuda", generator=gen(n)))).to(T(xt))
+    w = ops.F8Weight(w8.data_ptr(), ws.data_ptr(), n, k)
+    ref, mag = product64(x, w8, ws)
+    y = run_product(w, x, n, xt, yt, ldy=ldy)
+    check_product(y, ref, mag, k, yt)
+    assert torch.equal(run_product(w, x, n, xt, yt, ldy=ldy), y)
+    x[m - 2, k - 1] = float("nan")
+    z = run_product(w, x, n, xt, yt, ldy=ldy)
+    bad = torch.isnan(z)
+    assert bad[m - 2].all() and int(bad.sum()) == n
+    z[m - 2] = y[m - 2]
+    assert torch.equal(z, y)
+    w.sync()
+    w.close()
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n,ldy,tile", [c for c in MANY_TILES if c[1] == 784])
+def test_product_of_quantised_many_tiles(m, k, n, ldy, tile):
+    """The same with rows that are quantised already, inside wider ones."""
+    import torch
+    w8, ws = make_f8(n, k, m)
+    w = ops.F8Weight(w8.data_ptr(), ws.data_ptr(), n, k)
+    x = torch.randn(m, k, device="cuda", generator=gen(m))
+    q = torch.empty(m, k, device="cuda", dtype=torch.uint8)
+    s = torch.empty(-(-k // 128), m, device="cuda")
+    ops.f8_quantize_device(x.data_ptr(), "f32", m, k, q.data_ptr(), s.data_ptr(), stream=stream())
+    wide = torch.full((m, k + 32), 0x7F, device="cuda", dtype=torch.uint8)  # NaN behind the rows
+    wide[:, :k] = q
+    s *= 1.3
+    ref, mag = product64_q(q.view(torch.float8_e4m3fn).double(), s.double(), w8, ws)
+    check_product(run_product(w, wide[:, :k], n, "e4m3", "f16", ldy=ldy, scales=s), ref, mag, k, "f16")
+    w.close()
+
+
+# ------------------------------------------------ head norms of many heads --
+
+@gpu
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("pairing", ["interleaved", "half"])
+@pytest.mark.parametrize("t,hq,hk,d,rot", [(5003, 8, 8, 64, 64), (5003, 16, 8, 64, 48), (40011, 8, 8, 32, 32),
+                                           (20011, 16, 8, 128, 96), (30011, 8, 8, 128, 128), (9001, 16, 8, 256, 256),
+                                           (12001, 32, 8, 96, 64), (20011, 12, 9, 128, 96), (40011, 7, 13, 64, 64)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_qk_norm_many_heads(name, pairing, t, hq, hk, d, rot, packed):
+    """Eight and four heads a lane, below and above the size of the L2, into
+    other rows and in place inside packed ones with values behind."""
+    import torch
+    g = gen(t + d)
+    wide = (hq + 2 * hk) * d if packed else (hq + hk) * d
+    rows = torch.randn(t + 1, wide, device="cuda", generator=g).to(T(name))
+    before = rows.clone()
+    q, k = rows[:t, :hq * d], rows[:t, hq * d:(hq + hk) * d]
+    qw, kw = (1 + 0.3 * torch.randn(d, device="cuda", generator=g) for _ in range(2))
+    pos = torch.randint(0, 4000, (t,), device="cuda", generator=g, dtype=torch.int32)
+    qo, ko = (q, k) if packed else (torch.full((t, h * d), 9.0, device="cuda", dtype=T(name)) for h in (hq, hk))
+    r = ops.Rope(4000, rot, 10000.0, pairing)
+    r.qk_norm_device(name, t, hq, hk, d, q.data_ptr(), k.data_ptr(), pos.data_ptr(), qo.data_ptr(), ko.data_ptr(), wide,
+                     wide, qo.stride(0), ko.stride(0), qw.data_ptr(), kw.data_ptr(), 1e-6, stream())
+    r.sync()
+    for got, first, heads, w in ((qo, 0, hq, qw), (ko, hq * d, hk, kw)):
+        for a in range(0, t, 8192):  # the reference in 64 bits, a part at a time
+            x = before[a:min(t, a + 8192), first:first + heads * d]
+            check_qk(got[a:a + 8192].contiguous(), qk64(x, heads, d, rot, pairing, w, pos[a:a + 8192], 10000.0, 1e-6), name)
+    assert torch.equal(rows[t], before[t])
+    assert torch.equal(rows[:, (hq + hk) * d:], before[:, (hq + hk) * d:])
+    if not packed:
+        assert torch.equal(rows, before)
+    r.close()
