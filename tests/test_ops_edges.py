@@ -6,6 +6,10 @@ Rows far apart give the bits of the same rows packed.  The wide weight's
 products are sums of at most 64 small integers, exact in float32.  Attention
 has the tolerance of test_ops.py.
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -186,3 +190,62 @@ def test_rows_and_sequences_that_are_refused():
     for nseq in ((1 << 30) + 1, 1 << 32):
         expect_einval(lambda: a.run_device("f16", p, p, p, p, nseq, 2, 0, p, stream=stream()))
     a.close()
+
+
+FIRST_CALLS = """
+import numpy as np, torch
+from llm_embed_b200 import ops
+t, h, d = %d, 2, 64
+W = 2 * h * d
+g = torch.Generator("cuda").manual_seed(1)
+x = torch.randn(t, W, device="cuda", generator=g).half()
+w = ops.F8Weight.from_float(np.random.default_rng(1).standard_normal((3 * W, W)).astype(np.float32) / 16)
+rope, att = ops.Rope(t, d), ops.DiffAttention(h, h, d, np.zeros((4, d), np.float32), 0.5)
+pos = torch.arange(t, device="cuda", dtype=torch.int32)
+offs = torch.tensor([0, t // 2, t], device="cuda", dtype=torch.int32)
+work = torch.empty(w.workspace_bytes(t, "f16"), device="cuda", dtype=torch.uint8)
+qkv, out = (torch.zeros(t, n, device="cuda", dtype=torch.float16) for n in (3 * W, W))
+q8, s8 = torch.zeros(t, W, device="cuda", dtype=torch.uint8), torch.zeros(2, t, device="cuda")
+
+def layer(s):
+    ops.f8_quantize_device(x.data_ptr(), "f16", t, W, q8.data_ptr(), s8.data_ptr(), stream=s)
+    w.matmul_device(x.data_ptr(), t, qkv.data_ptr(), d_work=work.data_ptr(), work_bytes=work.numel(), stream=s)
+    q, k, v = (qkv.data_ptr() + 2 * W * i for i in range(3))
+    rope.qk_norm_device("f16", t, 2 * h, 2 * h, d, q, k, pos.data_ptr(), q, k, 3 * W, 3 * W, 3 * W, 3 * W, stream=s)
+    att.run_device("f16", q, k, v, offs.data_ptr(), 2, t, %d, out.data_ptr(), 3 * W, 3 * W, 3 * W, stream=s)
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):  # the process's first call of each
+    layer(torch.cuda.current_stream().cuda_stream)
+graph.replay()
+torch.cuda.synchronize()
+got = [y.clone() for y in (q8, s8, qkv, out)]
+for y in (q8, s8, qkv, out):
+    y.zero_()
+layer(ops.LEGACY_STREAM)
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, (q8, s8, qkv, out))) and float(out.abs().max()) > 0
+# Other sequences in the same graph: offsets are read at each replay.
+offs.copy_(torch.tensor([0, 1, t]))
+graph.replay()
+torch.cuda.synchronize()
+got = out.clone()
+layer(ops.LEGACY_STREAM)
+torch.cuda.synchronize()
+assert torch.equal(got, out)
+for hnd in (w, rope, att):
+    hnd.sync()
+print("same")
+"""
+
+
+@gpu
+@pytest.mark.parametrize("t,hint", [(6, 6), (50, 64), (100, 128), (700, 0)])
+def test_first_calls_of_a_process_are_captured(t, hint):
+    """A graph that holds the first call of every operator, replayed on other
+    offsets; in a process of its own, whose kernels are not loaded yet."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS % (t, hint)], cwd=root, capture_output=True, text=True,
+                       timeout=300, env=dict(os.environ, PYTHONPATH=root))
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
