@@ -213,8 +213,8 @@ int le_f8_quantize_device(int dev, int x_type, const void* d_x, int64_t ldx, int
 
 /* An e4m3 weight with a scale for each block of 128 x 128:
  *   y[m][n] = sum_b xs[b][m] ws[n/128][b] sum_{k in block b} xq[m][k] wq[n][k]
- * with the products of a block summed on the tensor cores and the blocks in
- * float32, rounded once to y's type.  N from 1, K a multiple of 16 (the last
+ * with the products of a block summed on the tensor cores, xs ws and the sum over
+ * the blocks in float32, rounded once to y's type.  N from 1, K a multiple of 16 (the last
  * block may be short), M from 0, each to 2^30. */
 typedef struct le_f8weight le_f8weight;
 /* wq [N][K] bytes and scales [ceil(N/128)][ceil(K/128)] (any float32), host
@@ -251,7 +251,7 @@ int le_f8weight_free(le_f8weight* w);
  *   u = x / sqrt(mean(x^2) + eps) * w over a head's columns, then
  *   (u_a, u_b) -> (u_a c - u_b s, u_a s + u_b c) for the pairs of its first
  * rot_dim columns, c and s of the angle position * base^(-2i / rot_dim) from a
- * table computed in 64 bits.  Pairs: (2i, 2i+1) with LE_ROPE_INTERLEAVED (the
+ * table computed in 64 bits; squares and their sum are float32.  Pairs: (2i, 2i+1) with LE_ROPE_INTERLEAVED (the
  * encoder's own, ops_simd.go:127-137), (i, i + rot_dim/2) with LE_ROPE_HALF. */
 #define LE_ROPE_INTERLEAVED 0
 #define LE_ROPE_HALF 1
@@ -295,7 +295,8 @@ typedef struct {
   int64_t q_stride, k_stride, v_stride, out_stride; /* elements, multiples of 8; 0 = packed */
   int32_t type;            /* LE_DT_F16 or LE_DT_BF16; pointers 16-byte aligned */
   int32_t nseq, n_tokens;
-  int32_t max_len;         /* longest sequence if known, else 0: only chooses the kernel */
+  int32_t max_len;         /* longest sequence if known, else 0: only chooses the kernel (all are
+                            * right for any length, within the rounding of weights to `type`) */
 } le_diffattn_args;
 /* Offsets that descend or leave [0, n_tokens] are reported by
  * le_diffattn_sync; no row outside [0, n_tokens) is then read or written, but

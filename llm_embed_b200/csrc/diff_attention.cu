@@ -14,6 +14,8 @@
 // the upper part of fp16's range); the sums are not.  Longer sequences (a caller whose hint of the longest was too
 // small) take the same steps block by block, in two passes: maxima and sums,
 // then weights and values.
+// Spilled registers: none in the 64-row kernels' own path, 44 to 80 bytes in the
+// 128-row ones (both maps of 128 keys), the rest in that of longer sequences.
 // Keys past the sequence get weight 0 and their values are zeros in shared
 // memory, whatever the rows behind hold.
 #include <mutex>

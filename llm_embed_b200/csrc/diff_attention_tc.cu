@@ -22,7 +22,7 @@
 // 64, bf16: 203 us (902 TFLOP/s; the exponentials alone 105 us at 1.9 GHz).  Of
 // 1860 clocks that a block of 64 keys takes a map's warps, 630 are exponentials
 // (512 at least), 390 the maximum and scaling, 270 packing and writing the
-// weights, 320 the wait for scores, 170 the turn.  256 texts of 16 to 128: 49 us;
+// weights, 320 the wait for scores, 170 the turn.  256 texts of 16 to 128: 51 us;
 // the longest part of a tile of one or two key blocks is its epilogue.
 //
 //   warp 0      producer: TMA loads of Q (two stages), K and V (four each)
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   // 512 threads of 128 registers at launch: 56 + 2 * 128 + 200 = 4 * 128.  Short
   // tiles wait for the epilogue, whose 128 results a thread and two loads of 32
   // columns need the most (256 texts of 16 to 128: 54 us with 144 and 168
-  // registers, loads of 16 and weights in shared memory, 49 us so).
+  // registers, loads of 16 and weights in shared memory, 49 to 51 us so).
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 3) {

@@ -1,7 +1,7 @@
 // Eight-bit product for few tokens (mma.sync m16n8k32 e4m3, sm_100a):
 //   y[m][n] = sum_b xs[b][m] ws[n/128][b] sum_{k in block b} xq[m][k] wq[n][k]
-// with the activations quantised on the fly (f8.cuh), so a call is one launch
-// and reads each weight byte once.  Bound by the weight's bytes, or by latency
+// with the activations of up to 8 rows quantised on the fly (f8.cuh), so that
+// such a call is one launch; each weight byte is read once.  Bound by the weight's bytes, or by latency
 // when those are few (1 x 768 . 2304: 1.8 us; 24 x 4096 . 4096: 6.5 us, 2.6 TB/s
 // of weight, behind a quantiser of 1.5 us).
 //

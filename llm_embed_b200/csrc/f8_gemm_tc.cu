@@ -13,11 +13,12 @@
 // costs, the tensor cores need 512 and the warps that add 256 for their fmas,
 // the rest is the way from MMA to addition and back.  Without the loads of the
 // sums it would be 121 us where it is 129 (8192 x 4096 . 4096), without the
-// wait for the accumulator 90.  Measured with rows that are quantised already:
-//   8192 x 4096 . 4096    129 us  2.13 PFLOP/s
-//   32768 x 768 . 2304     71 us  1.63 PFLOP/s
-//   512 x 4096 . 4096      15 us
-//   333 x 768 . 2304      4.8 us
+// wait for the accumulator 90.  Measured with rows that are quantised already,
+// 50 calls in a graph:
+//   8192 x 4096 . 4096    129 us  2.13 PFLOP/s (to 142 once the chip is at its power limit)
+//   32768 x 768 . 2304     70 us  1.66 PFLOP/s
+//   512 x 4096 . 4096    14.4 us  (12.6 before the narrow tiles' present form)
+//   333 x 768 . 2304      4.7 us
 //
 // Persistent kernel; tile = 128 * CG token rows x BN weight rows.  CG = 2: a
 // cluster of two CTAs computes it with one MMA of M = 256 (cta_group::2), each

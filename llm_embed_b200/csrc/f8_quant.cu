@@ -58,7 +58,9 @@ __global__ void __launch_bounds__(THREADS) quant_vec_kernel(const T* __restrict_
   }
 }
 
-// Any K, row stride and alignment: one warp per block of 128 columns.
+// Any K, row stride and alignment: one warp per block of 128 columns.  Bound by
+// its instructions, with single elements loaded and stored: 18431 x 4095 of bf16
+// in 94 us, 2.4 TB/s, where rows on 16 bytes take 38.
 template <class T>
 __global__ void __launch_bounds__(THREADS) quant_any_kernel(const T* __restrict__ x, long ldx, long items, int M,
                                                             int K, int KB, uint8_t* __restrict__ q,

@@ -137,7 +137,9 @@ __global__ void __launch_bounds__(THREADS) qk_norm_vec_kernel(QkNormParams p) {
 }
 
 // Any head size up to MAX_D, rotation and alignment: one warp per head
-// vector, staged through shared memory for the rotation's pairs.
+// vector, staged through shared memory for the rotation's pairs.  Bound by
+// instructions and latency, about the same for every head size (18431 tokens,
+// 12 + 12 heads of 50, 64 or 80: 229 us; 22 for 64 aligned columns).
 constexpr int MAX_D = 256;
 template <class T>
 __global__ void __launch_bounds__(THREADS) qk_norm_any_kernel(QkNormParams p) {
@@ -221,7 +223,8 @@ static cudaError_t launch_g(const QkNormParams& p, int n, cudaStream_t s) {
   // blocks of them; eight of the 2-byte types where both kinds come in eights
   // (32 + 8 heads of 128, bf16: 132 -> 121 us; 12 + 12 heads of 64 padded to 16:
   // 22.7 -> 26.4 us), past the L2's 126 MB with loads and stores that are not
-  // kept there (121 -> 114 us).
+  // kept there (121 -> 114 us).  Four a lane keeps them: 24 + 6 heads of 128 in
+  // 94 us, 5.4 TB/s; float32, 32 + 8 heads, 210 us, 6.4 TB/s.
   const long vectors = (long)n * (p.q_heads + p.k_heads);
   if (vectors < 148L * 16 * 4 * (THREADS / G)) return launch_vec<T, G, 1>(p, n, s);
   if constexpr (sizeof(T) == 2)
