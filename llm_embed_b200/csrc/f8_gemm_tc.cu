@@ -292,6 +292,9 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       const uint64_t a0 = sw128_desc(sbase + C::OFF_A), b0 = sw128_desc(sbase + C::OFF_B);
       uint32_t it = 0;
       bool ok = true;
+      // The rows come once the previous kernel has ended, however long that
+      // takes: the bounded waits for them begin there too.
+      pdl_wait();
       for (int tile = first; tile < total && ok; tile += step) {
         for (int kb = 0; kb < KB && ok; kb++, it++) {
           const uint32_t s = it % S, acc = it % NACC;

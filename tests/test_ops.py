@@ -1221,3 +1221,34 @@ def test_qk_norm_many_heads(name, pairing, t, hq, hk, d, rot, packed):
     if not packed:
         assert torch.equal(rows, before)
     r.close()
+
+
+@gpu
+@pytest.mark.parametrize("m", [300, 4225])
+def test_product_behind_a_long_kernel(m):
+    """The product's kernel starts while the one before it (seconds on one SM)
+    still runs, and waits for it without its own limits running out."""
+    import torch
+    n, d, k, cols = 51200, 32, 272, 2312
+    q = torch.zeros(n, 2 * d, device="cuda", dtype=torch.float16)
+    out = torch.empty_like(q)
+    offs = torch.tensor([0, n], device="cuda", dtype=torch.int32)
+    a = ops.DiffAttention(1, 1, d, np.zeros((4, d), np.float32), INIT, None)
+    w8, ws = make_f8(cols, k, m)
+    w = ops.F8Weight(w8.data_ptr(), ws.data_ptr(), cols, k)
+    x = torch.randn(m, k, device="cuda", generator=gen(m))
+    x8, xs = torch.empty(m, k, device="cuda", dtype=torch.uint8), torch.empty(3, m, device="cuda")
+    ops.f8_quantize_device(x.data_ptr(), "f32", m, k, x8.data_ptr(), xs.data_ptr(), stream=stream())
+    want = run_product(w, x8, cols, "e4m3", "f16", scales=xs)
+    y = torch.zeros(m, cols, device="cuda", dtype=torch.float16)
+    e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    torch.cuda.synchronize()
+    e[0].record()
+    a.run_device("f16", *(3 * [q.data_ptr()]), offs.data_ptr(), 1, n, 1, out.data_ptr(), stream=stream())
+    w.matmul_device(x8.data_ptr(), m, y.data_ptr(), "e4m3", "f16", d_x_scales=xs.data_ptr(), stream=stream())
+    e[1].record()
+    w.sync()
+    a.sync()
+    assert torch.equal(y, want) and e[0].elapsed_time(e[1]) > 2500  # the limit is 2 s
+    w.close()
+    a.close()
