@@ -1252,3 +1252,36 @@ def test_product_behind_a_long_kernel(m):
     assert torch.equal(y, want) and e[0].elapsed_time(e[1]) > 2500  # the limit is 2 s
     w.close()
     a.close()
+
+
+@gpu
+@pytest.mark.parametrize("m", [6, 24, 300, 5000])
+@pytest.mark.parametrize("ld", [256, 257])
+def test_chain_of_products(m, ld):
+    """Each product's result is the next one's input, in the same two buffers
+    (every kernel starts while the one before it ends): the bits of the same
+    calls one at a time."""
+    import torch
+    n = 256
+    w = ops.F8Weight.from_float(np.random.default_rng(m).standard_normal((n, n)).astype(np.float32) / 16)
+    x = torch.randn(m, n, device="cuda", generator=gen(m)).half()
+    work = torch.empty(w.workspace_bytes(m, "f16"), device="cuda", dtype=torch.uint8)
+
+    def chain(wait):
+        a, b = (torch.zeros(m, ld, device="cuda", dtype=torch.float16) for _ in range(2))
+        a[:, :n] = x
+        torch.cuda.synchronize()
+        for _ in range(60):
+            w.matmul_device(a.data_ptr(), m, b.data_ptr(), ldx=ld, ldy=ld, d_work=work.data_ptr(),
+                            work_bytes=work.numel(), stream=stream())
+            if wait:
+                torch.cuda.synchronize()
+            a, b = b, a
+        torch.cuda.synchronize()
+        return a[:, :n].clone()
+
+    want = chain(True)
+    assert torch.isfinite(want).all() and float(want.abs().max()) > 0
+    for _ in range(5):
+        assert torch.equal(chain(False), want)
+    w.close()
