@@ -43,7 +43,8 @@
 // multiple of 16 keys, and the values between (another sequence's, or
 // garbage) are overwritten with zeros in shared memory before it, so nothing
 // but the sequence's own rows reaches a result.  Query rows past it are not
-// stored.  Every mbarrier wait is bounded (WAIT_LIMIT_NS).
+// stored.  Every mbarrier wait is bounded (WAIT_LIMIT_NS); after one that ran out
+// the CTA lets its copies and MMAs end before it exits.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -648,6 +649,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
+    settle(abort_flag);
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }

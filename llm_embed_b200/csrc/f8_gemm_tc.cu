@@ -31,7 +31,8 @@
 //              rows go out through shared memory and TMA stores, or by plain
 //              stores where y's rows do not begin and end on 16 bytes
 // Rows and columns past M, N and K are zeros from TMA and are not stored.
-// Every mbarrier wait is bounded (WAIT_LIMIT_NS).
+// Every mbarrier wait is bounded (WAIT_LIMIT_NS); after one that ran out the CTA
+// lets its copies and MMAs end before it exits.
 #include <cudaTypedefs.h>
 
 #include <mutex>
@@ -431,6 +432,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
 
   tc_fence_before();
   __syncthreads();
+  if (warp == 1) settle(abort_flag);
   if constexpr (CG == 2) cluster_sync();  // the peer is done with this CTA's shared memory and TMEM
   if (warp == 1) {
     tc_fence_after();

@@ -103,6 +103,18 @@ __device__ __forceinline__ bool mbar_wait_impl(uint32_t bar, uint32_t parity, vo
   }
 }
 
+// For the warp that frees the TMEM, before the CTA exits: where a wait ran out,
+// copies and MMAs may be under way that nobody has waited for; they end within
+// microseconds and get 10 ms.
+__device__ __forceinline__ void settle(const volatile int* abort_flag) {
+  if (*abort_flag) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 10000000ull) {
+    }
+  }
+  __syncwarp();
+}
+
 // AND of `ok` over the dequant threads (named barrier 1): every thread of
 // the group takes the same branch, so no thread is left at a barrier.
 __device__ __forceinline__ bool dequant_group_all(bool ok, int nthreads) {
