@@ -687,6 +687,25 @@ def test_diff_attention_many_sequences(count, lo, hi, norm):
 
 
 @gpu
+@pytest.mark.parametrize("lens", [[9001, 300, 4097], [16385]])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("sharp", [0.5, 3.0])
+def test_diff_attention_long(lens, name, sharp):
+    """Thousands of keys, from nearly equal weights to a few that count."""
+    import torch
+    h, d = 2, 64
+    q, k, v, offs, t = make_diff(lens, h, 1, d, name, 11, sharp=sharp)
+    lam, val = lambdas(h, d, True, 3)
+    nw = torch.linspace(0.5, 1.5, 2 * d)
+    a = ops.DiffAttention(h, 1, d, lam, INIT, nw.numpy(), 1e-5)
+    out = run_diff(a, q, k, v, offs, t, h, d, name)
+    a.sync()
+    ref, mag = diff64(q, k, v, offs.tolist(), h, 1, d, val, INIT, nw.cuda(), 1e-5)
+    check_diff(out, ref, mag, name)
+    a.close()
+
+
+@gpu
 @pytest.mark.parametrize("lens", [[5], [60, 70], [200, 130], [600]])
 @pytest.mark.parametrize("name", ["f16", "bf16"])
 def test_diff_attention_ignores_other_rows(lens, name):
